@@ -188,9 +188,9 @@ def run_own(state):
         dx, dr, dw = torch.autograd.grad((y, h), (state["x"], state["r"], state["w"]), (state["dy"], state["dh"]))
         return y.detach(), h.detach(), dx, dr, dw
     if case["op"] == "clip":
-        from instancerefer_amd.optim import clip_grad_norm_
+        from instancerefer_amd.optim import clip_grads_
         torch._foreach_copy_(state["grads"], state["fresh"])  # a backward pass leaves new gradients in place
-        norm = clip_grad_norm_(state["grads"], state["max_norm"])
+        norm = clip_grads_(state["grads"], state["max_norm"])
         return [norm] + state["grads"]
     if case["op"] == "step":
         opt = state["opt"]
