@@ -606,6 +606,61 @@ int irx_adam_step(float* params, const float* grads, float* exp_avg, float* exp_
                   float beta1, float beta2, float eps, float weight_decay, int step, float grad_scale,
                   void* stream);
 
+/* Global gradient norm over many tensors, and clipping: norm = sqrt(sum g^2) (inf_norm != 0: max |g|), factor = min(1, max_norm /
+ * (norm + 1e-6)), NaN if the norm is. The reference trains without clipping (lib/solver.py:200-205). Sums are 64 bits, in a fixed order.
+ *
+ * irx_clip_grads: scales n_tensors tensors in place and writes the norm BEFORE clipping to norm[0] (device float). Host arrays of device
+ *   pointers, types (0 float32, 1 bf16, 2 fp16) and element counts; a tensor is one contiguous range, two tensors must not share memory.
+ * irx_grad_norm_parts + irx_adam_step_clip: the same for ONE flat float32 buffer inside the optimizer: the first leaves partial sums of
+ *   grads[0, n) in workspace, the second is irx_adam_step with the gradients multiplied by grad_scale * factor as they are read (no
+ *   clipped gradients are written); norm_parts = that workspace, norm_values = that n, and the norm counts grad_scale. norm (may be
+ *   NULL): device float. With a factor of 1 it computes what irx_adam_step does. */
+size_t irx_clip_grads_workspace_bytes(const unsigned long long* counts_host, int n_tensors);
+int irx_clip_grads(void* const* grads_host, const int* types_host, const unsigned long long* counts_host, int n_tensors, int inf_norm,
+                   float max_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream);
+size_t irx_grad_norm_workspace_bytes(size_t n);
+int irx_grad_norm_parts(const float* grads, size_t n, int inf_norm, void* workspace, size_t workspace_bytes, void* stream);
+int irx_adam_step_clip(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, size_t n, float lr, float beta1,
+                       float beta2, float eps, float weight_decay, int step, float grad_scale, const void* norm_parts,
+                       size_t norm_values, int inf_norm, float max_norm, float* norm, void* stream);
+
+/* Root-mean-square norm with the residual's addition. Types: 0 float32, 1 bf16, 2 fp16; weight float32 (weight_f32) or the same type.
+ *   fwd: h = x + residual rounded to the type (residual NULL: h is x and is not written), rstd = 1 / sqrt(mean(h^2) + eps) over cols,
+ *        y = h * rstd * weight. rstd float32 [rows] (may be NULL).
+ *   bwd: dx = dh + rstd * (weight * dy - h rstd * mean(weight * dy * h rstd)) (dh NULL: 0) — the gradient of x and of the residual —
+ *        and dweight = sum over rows of dy * h rstd. dx may be dh or dy. Deterministic. rows < 2^31, any cols. */
+int irx_rms_norm_fwd(const void* x, const void* residual, const void* weight, int weight_f32, long long rows, int cols, int dtype,
+                     float eps, void* y, void* h, float* rstd, void* stream);
+size_t irx_rms_norm_bwd_workspace_bytes(long long rows, int cols, int dtype);
+int irx_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* weight, int weight_f32, const float* rstd, long long rows,
+                     int cols, int dtype, void* dx, void* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention over packed sequences (beside the GRU of the language encoder, models/lang_module.py:53-57, which packs its descriptions too).
+ * q [tq][heads][dim], k and v [tk][kv_heads][dim], query head h reads key / value head h / (heads / kv_heads); each with its own row
+ * and head strides in ELEMENTS (dim contiguous; rows and heads start on 16 bytes). cu_q, cu_k int32 [batch + 1] (device): sequence b is
+ * rows cu[b] .. cu[b + 1]; rows outside every sequence get zeros. dim 32, 64 or 128; dtype 0 float32, 1 bf16, 2 fp16.
+ *   score_ij = scale * q_i . k_j + bias;  visible: every key j of the same sequence, with causal != 0 only j <= i + Lk - Lq
+ *   (the last query sees the last key). A row that sees nothing gives zeros and takes no gradient.
+ *   bias (table != NULL) = table[map[far + clamp(j - (i + Lk - Lq), -far, far)]][h]; table [buckets][heads] float32 (table_f32) or the
+ *   tensors' type, map int32 [2 far + 1] (device, far <= 512).
+ * out, dq [tq][heads][dim], dk, dv [tk][kv_heads][dim] contiguous; stats float32 [heads][tq][2] is what the backward needs of the
+ * forward (NULL: not written); dtable like table. Offsets are read on the device only: no length has to be known on the host.
+ * Deterministic. irx_attn_packed_bwd_workspace_bytes: far = -1 without a bias table. */
+size_t irx_attn_packed_fwd_workspace_bytes(int tq, int tk, int batch, int heads, int dim);
+int irx_attn_packed_fwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
+                        const void* v, long long v_row, long long v_head, const int32_t* cu_q, const int32_t* cu_k, int batch, int tq,
+                        int tk, int heads, int kv_heads, int dim, int dtype, float scale, int causal, const void* table,
+                        int table_f32, const int32_t* map, int buckets, int far, void* out, float* stats, void* workspace,
+                        size_t workspace_bytes, void* stream);
+size_t irx_attn_packed_bwd_workspace_bytes(int tq, int batch, int heads, int far);
+int irx_attn_packed_bwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
+                        const void* v, long long v_row, long long v_head, const void* dout, long long do_row, long long do_head,
+                        const void* out, const float* stats, const int32_t* cu_q, const int32_t* cu_k, int batch, int tq, int tk,
+                        int heads, int kv_heads, int dim, int dtype, float scale, int causal, const void* table, int table_f32,
+                        const int32_t* map, int buckets, int far, void* dq, void* dk, void* dv, void* dtable, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+
 /* ---- instance graph ------------------------------------------------------------------- */
 
 /* torch_cluster.knn(x=support, y=query, k, batch_x, batch_y) (models/basic_blocks.py:120):

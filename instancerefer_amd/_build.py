@@ -10,8 +10,8 @@ from concurrent.futures import ThreadPoolExecutor
 
 CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 LIB_PATH = os.environ.get("IRX_LIB_PATH") or os.path.join(CSRC, "libirx.so")   # override: dev-only instrumented builds
-SOURCES = ["irx_coords.hip", "irx_sort.hip", "irx_sched.hip", "irx_spconv.hip", "irx_spconv2.hip", "irx_spconv3.hip", "irx_pairs.hip", "irx_encoder.hip", "irx_stem.hip", "irx_norm.hip", "irx_pool.hip", "irx_match.hip", "irx_mlp.hip", "irx_input.hip", "irx_gru.hip", "irx_optim.hip", "irx_labels.hip", "irx_project.hip", "irx_edgeconv.hip"]
-HEADERS = ["irx_common.h", os.path.join("..", "..", "include", "irx.h")]
+SOURCES = ["irx_coords.hip", "irx_sort.hip", "irx_sched.hip", "irx_spconv.hip", "irx_spconv2.hip", "irx_spconv3.hip", "irx_pairs.hip", "irx_encoder.hip", "irx_stem.hip", "irx_norm.hip", "irx_pool.hip", "irx_match.hip", "irx_mlp.hip", "irx_input.hip", "irx_gru.hip", "irx_optim.hip", "irx_labels.hip", "irx_project.hip", "irx_edgeconv.hip", "irx_rmsnorm.hip", "irx_attn.hip", "irx_attn_bwd.hip"]
+HEADERS = ["irx_common.h", "irx_attn.h", os.path.join("..", "..", "include", "irx.h")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -packed-fp32-ops: no v_pk_*_f32 (the compiler makes them out of ordinary float code; some of their forms have given wrong results now
 # and then on this hardware). The host pass does not know the feature and says so: harmless.
@@ -81,7 +81,7 @@ def _build_locked(objdir, verbose):
 # A Python extension module compiled against the torch headers with g++ (host code only: it calls libirx through function
 # addresses and never touches HIP). In-tree like libirx.so, so it travels to the GPU box with the snapshot.
 NODES_SRC = os.path.join(CSRC, "torch_nodes.cpp")
-NODES_SRCS = [NODES_SRC, os.path.join(CSRC, "heads_nodes.cpp")]       # heads_nodes.cpp: one node per head (round 6)
+NODES_SRCS = [NODES_SRC, os.path.join(CSRC, "heads_nodes.cpp"), os.path.join(CSRC, "text_nodes.cpp")]   # one node per operator, per head; text encoder
 NODES_HDRS = [os.path.join(CSRC, "torch_nodes.h")]
 NODES_PATH = os.path.join(CSRC, "_irx_nodes.so")
 CXX = os.environ.get("CXX", "g++")

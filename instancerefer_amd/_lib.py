@@ -17,6 +17,7 @@ _I = _c.c_int
 _Z = _c.c_size_t
 _F = _c.c_float
 _D = _c.c_double
+_L = _c.c_longlong
 
 # name -> (restype, argtypes) : mirrors include/irx.h one to one
 _SIGNATURES = {
@@ -112,6 +113,20 @@ _SIGNATURES = {
     "irx_edgeconv_max_fwd": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P]),
     "irx_edgeconv_max_bwd": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _Z, _P]),
     "irx_iou_labels": (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P]),
+    "irx_clip_grads_workspace_bytes": (_Z, [_P, _I]),
+    "irx_clip_grads": (_I, [_P, _P, _P, _I, _I, _F, _P, _P, _Z, _P]),
+    "irx_grad_norm_workspace_bytes": (_Z, [_Z]),
+    "irx_grad_norm_parts": (_I, [_P, _Z, _I, _P, _Z, _P]),
+    "irx_adam_step_clip": (_I, [_P, _P, _P, _P, _Z, _F, _F, _F, _F, _F, _I, _F, _P, _Z, _I, _F, _P, _P]),
+    "irx_rms_norm_fwd": (_I, [_P, _P, _P, _I, _L, _I, _I, _F, _P, _P, _P, _P]),
+    "irx_rms_norm_bwd_workspace_bytes": (_Z, [_L, _I, _I]),
+    "irx_rms_norm_bwd": (_I, [_P, _P, _P, _P, _I, _P, _L, _I, _I, _P, _P, _P, _Z, _P]),
+    "irx_attn_packed_fwd_workspace_bytes": (_Z, [_I, _I, _I, _I, _I]),
+    "irx_attn_packed_fwd": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _I, _P, _I, _I, _P, _P, _P,
+                                 _Z, _P]),
+    "irx_attn_packed_bwd_workspace_bytes": (_Z, [_I, _I, _I, _I]),
+    "irx_attn_packed_bwd": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _I, _P,
+                                 _I, _I, _P, _P, _P, _P, _P, _Z, _P]),
     "irx_eval_select": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P]),
 }
 

@@ -61,3 +61,20 @@ def _load_locked():
                       "Python / ATen path; rebuild with `python -m instancerefer_amd._build`" % (type(e).__name__, e), RuntimeWarning)
         return None
     return mod
+
+
+def refuse_foreign_leaves(who, leaves):
+    """Called under a graph capture, before a node on `leaves` is made or run backward: raises when one of them still belongs to an eager
+    graph of another stream. Its backward would make that stream wait inside the capture, which ends the process when the capture ends."""
+    mod = load()
+    if mod is None:
+        raise RuntimeError("%s: gradients can be captured into a graph only with csrc/_irx_nodes.so (python -m instancerefer_amd._build)" % who)
+    i = mod.foreign_leaf(list(leaves))
+    if i >= 0:
+        raise RuntimeError("%s: a backward pass cannot be captured while an eager graph of the same leaves lives (input %d was used on "
+                           "another stream): drop that graph's outputs first, or run the warm-up on the capture's stream" % (who, i))
+
+
+def leaves_of(ctx):
+    """the leaf tensors right behind a Python autograd.Function's node"""
+    return [n.variable for n, _ in ctx.next_functions if n is not None and hasattr(n, "variable")]

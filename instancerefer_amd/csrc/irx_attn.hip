@@ -1,0 +1,302 @@
+// irx_attn.hip — attention over packed sequences, forward (grouped heads, causal or full, learned relative position bias by buckets).
+//
+// One pass over the keys with the running maximum and sum of each row: o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m). A workgroup owns 128
+// query rows of one head (four waves, 32 rows each); tiles of 64 keys and their values pass through LDS. The scores are computed transposed
+// (keys down, queries across), so that a row of the softmax is one lane pair and the weights are the next product's operand as they are
+// (irx_attn.h); the output is accumulated transposed as well and its rescaling is one factor per lane.
+// Exponents are base 2 (scale * log2 e is folded into one multiply-add per score); scores, weights' sums and the output are 32 bits, the
+// weights are rounded to the operand type for the second product (a relative 2^-9 / 2^-12 per weight, below the output's own rounding).
+#include "irx_attn.h"
+
+template <class T, int D, bool BIAS>
+__global__ __launch_bounds__(256, (T::ESZ == 4 && D == 128) ? 1 : 2) void k_attn_fwd(AtParams P, int total) {
+  typedef AtTile<T, D> Tile;
+  typedef typename T::F F;
+  typedef typename T::S S;
+  constexpr int STEPS = D / 16, BLOCKS = D / 32;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  unsigned char* lk_ = smem;
+  unsigned char* lv_ = smem + Tile::BYTES;
+  float* sb = reinterpret_cast<float*>(smem + 2 * Tile::BYTES);
+
+  // consecutive workgroups go to the 8 XCDs in turn: give each XCD a contiguous run of (head, slot), so that a head's keys and values are
+  // read through one L2; the last slots of a sequence, the longest ones under a causal mask, first
+  const int per = gridDim.x >> 3;
+  const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (id >= total) return;
+  const int slot = P.slots - 1 - id % P.slots;
+  const int hs = id / P.slots, head = hs % P.heads, part = hs / P.heads;
+
+  int first;
+  const AtSpan sp = at_span(P.cu_q, P.batch, P.tq, IRX_ATTN_BM, slot, &first);
+  if (sp.begin >= sp.end) return;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int kb = 0, ke = 0;
+  if (sp.seq >= 0) {
+    kb = at_edge(P.cu_k, P.batch, P.tk, sp.seq + 1);
+    ke = at_edge(P.cu_k, P.batch, P.tk, sp.seq + 2);
+  }
+  const int lk = ke > kb ? ke - kb : 0, off = lk - (sp.end - first);
+  const int row0 = sp.begin + wave * 32;
+  const int q = row0 + (lane & 31);
+  const bool mine = q < sp.end;
+  const int i0 = row0 - first;                                           // index in the sequence of this wave's first row
+  const int lim = P.causal ? min(lk, i0 + (lane & 31) + 1 + off) : lk;   // keys [0, lim) are visible to this lane's row
+  const int wave_full = P.causal ? min(lk, i0 + 1 + off) : lk;           // ... to every row of the wave
+  const int wave_any = row0 >= sp.end ? 0 : (P.causal ? min(lk, min(i0 + 32, sp.end - first) + off) : lk);
+  const int block_any = P.causal ? min(lk, min(sp.begin + IRX_ATTN_BM, sp.end) - first + off) : lk;
+  int t0 = 0, t1 = (max(block_any, 0) + IRX_ATTN_BN - 1) / IRX_ATTN_BN;
+  if (P.splits > 1) {
+    const int n = t1;
+    t0 = (int)((long long)n * part / P.splits);
+    t1 = (int)((long long)n * (part + 1) / P.splits);
+  }
+  const int kvh = head / (P.heads / P.kv_heads);
+  const S* kp = reinterpret_cast<const S*>(P.k.p) + kb * P.k.st + kvh * P.k.sh;
+  const S* vp = reinterpret_cast<const S*>(P.v.p) + kb * P.v.st + kvh * P.v.sh;
+  const float c1 = P.scale * IRX_LOG2E;
+
+  F qf[STEPS];
+  {
+    const S* qp = reinterpret_cast<const S*>(P.q.p) + q * P.q.st + head * P.q.sh + 8 * half;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) qf[s] = mine ? at_ldg<T>(qp + 16 * s) : at_zero<T>();
+  }
+  if constexpr (BIAS) at_load_bias<T>(sb, P, head);
+
+  at_f32x16 acc[BLOCKS];
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
+  float m = -INFINITY, l = 0.f;               // l: this lane's half of the row only
+
+  for (int t = t0; t < t1; ++t) {
+    const int k0 = t * IRX_ATTN_BN;
+    __syncthreads();
+    Tile::template copy_in<256>(lk_, kp + k0 * P.k.st, P.k.st, lk - k0);
+    Tile::template copy_in<256>(lv_, vp + k0 * P.v.st, P.v.st, lk - k0);
+    __syncthreads();
+    if (k0 >= wave_any) continue;
+    float s[32];
+#pragma unroll
+    for (int kb2 = 0; kb2 < 2; ++kb2) {
+      at_f32x16 x;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = 0.f;
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st) x = at_mma(Tile::row_frag(lk_, 32 * kb2, st), qf[st], x);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[16 * kb2 + i] = x[i];
+    }
+    // key of register i: k0 + 8 (i / 4) + 4 half + i % 4
+    if constexpr (BIAS) {
+      const int lo = k0 - (i0 + 31 + off), hi = k0 + IRX_ATTN_BN - 1 - (i0 + off);      // distances key - query in this tile
+      if (hi <= -P.far || lo >= P.far) {
+        const float b = sb[hi <= -P.far ? 0 : 2 * P.far];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s[i] = __builtin_fmaf(s[i], c1, b);
+      } else {
+        const int d0 = k0 + 4 * half - (i0 + (lane & 31) + off);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int d = d0 + 8 * (i >> 2) + (i & 3);
+          s[i] = __builtin_fmaf(s[i], c1, sb[min(max(d, -P.far), P.far) + P.far]);
+        }
+      }
+    }
+    if (k0 + IRX_ATTN_BN > wave_full) {
+      const int left = lim - k0 - 4 * half;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) s[i] = 8 * (i >> 2) + (i & 3) < left ? s[i] : -INFINITY;
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i]);
+    mx = fmaxf(mx, at_other_half(mx));
+    if constexpr (!BIAS) mx *= c1;                                       // c1 > 0
+    // the running maximum moves only when a row outgrows it by 2^8: weights stay below 256, and most tiles rescale nothing
+    if (__any(mx > m + 8.f || m == -INFINITY)) {
+      const float mn = fmaxf(m, mx);
+      const float a = mn == -INFINITY ? 1.f : at_exp2(m - mn);
+      m = mn;
+      l *= a;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[b][i] *= a;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      s[i] = at_exp2(BIAS ? s[i] - ms : __builtin_fmaf(s[i], c1, -ms));
+      sum += s[i];
+    }
+    l += sum;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const F p = at_pack<T>(s + 8 * ks);
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) acc[b] = at_mma(Tile::col_frag(lv_, 16 * ks, b), p, acc[b]);
+    }
+  }
+  if (!mine) return;
+  l += at_other_half(l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;                            // a row that sees nothing: zeros
+  if (P.splits > 1) {
+    const size_t r = ((size_t)part * P.heads + head) * P.tq + q;
+    float* o = P.so + r * D + 4 * half;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        at_st4<AtF32>(o + 32 * b + 8 * g, acc[b][4 * g] * inv, acc[b][4 * g + 1] * inv, acc[b][4 * g + 2] * inv, acc[b][4 * g + 3] * inv);
+    if (half == 0) {
+      P.sst[2 * r] = m;
+      P.sst[2 * r + 1] = l;
+    }
+    return;
+  }
+  S* o = reinterpret_cast<S*>(P.dst) + ((size_t)q * P.heads + head) * D + 4 * half;
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      at_st4<T>(o + 32 * b + 8 * g, acc[b][4 * g] * inv, acc[b][4 * g + 1] * inv, acc[b][4 * g + 2] * inv, acc[b][4 * g + 3] * inv);
+  if (P.wstats && half == 0) {
+    float* st = P.wstats + ((size_t)head * P.tq + q) * 2;
+    st[0] = m == -INFINITY ? 0.f : m;
+    st[1] = inv;
+  }
+}
+
+// joins the parts of a row: o = sum_p w_p o_p / sum_p w_p, w_p = l_p 2^(m_p - max m); parts in their order, so always the same result
+template <class T, int D>
+__global__ __launch_bounds__(256) void k_attn_join(AtParams P) {
+  constexpr int PER = D / 4;
+  const size_t n = (size_t)P.heads * P.tq * PER, at = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= n) return;
+  const size_t row = at / PER;                                           // head * tq + q
+  const int d = (int)(at % PER) * 4;
+  const size_t rows = (size_t)P.heads * P.tq;
+  float M = -INFINITY;
+  for (int p = 0; p < P.splits; ++p) M = fmaxf(M, P.sst[2 * (p * rows + row)]);
+  const float Ms = M == -INFINITY ? 0.f : M;
+  float L = 0.f;
+  at_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < P.splits; ++p) {
+    const float l = P.sst[2 * (p * rows + row) + 1];
+    if (l == 0.f) continue;
+    const float w = l * at_exp2(P.sst[2 * (p * rows + row)] - Ms);
+    const at_f32x4 x = *reinterpret_cast<const at_f32x4*>(P.so + (p * rows + row) * D + d);
+    L += w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(w, x[i], o[i]);
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const size_t head = row / P.tq, q = row % P.tq;
+  at_st4<T>(reinterpret_cast<typename T::S*>(P.dst) + (q * P.heads + head) * D + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  if (P.wstats && d == 0) {
+    P.wstats[2 * row] = Ms;
+    P.wstats[2 * row + 1] = inv;
+  }
+}
+
+template <class T, int D, bool BIAS> static int launch_fwd(const AtParams& P, hipStream_t st) {
+  const size_t lds = 2 * AtTile<T, D>::BYTES + (BIAS ? sizeof(float) * (2 * P.far + 1) : 0);
+  const long long total = (long long)P.slots * P.heads * P.splits;
+  const unsigned grid = (unsigned)((total + 7) / 8 * 8);
+  if (int rc = at_want_lds(reinterpret_cast<const void*>(&k_attn_fwd<T, D, BIAS>), lds, "irx_attn_packed_fwd")) return rc;
+  k_attn_fwd<T, D, BIAS><<<grid, 256, lds, st>>>(P, (int)total);
+  IRX_CHECK_LAUNCH("irx_attn_packed_fwd");
+  if (P.splits > 1) {
+    const size_t n = (size_t)P.heads * P.tq * (D / 4);
+    k_attn_join<T, D><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(P);
+    IRX_CHECK_LAUNCH("irx_attn_packed_fwd(join)");
+  }
+  return IRX_OK;
+}
+template <class T, int D> static int launch_fwd_b(const AtParams& P, hipStream_t st) {
+  return P.table ? launch_fwd<T, D, true>(P, st) : launch_fwd<T, D, false>(P, st);
+}
+template <class T> static int launch_fwd_d(const AtParams& P, int dim, hipStream_t st) {
+  return dim == 32 ? launch_fwd_b<T, 32>(P, st) : dim == 64 ? launch_fwd_b<T, 64>(P, st) : launch_fwd_b<T, 128>(P, st);
+}
+
+int at_check(const char* who, const AtParams& P, int dim, int dtype, int elem) {
+  IRX_REQUIRE(dtype >= IRX_ATTN_F32 && dtype <= IRX_ATTN_F16, "%s: type %d (0 float32, 1 bfloat16, 2 float16)", who, dtype);
+  IRX_REQUIRE(dim == 32 || dim == 64 || dim == 128, "%s: head dimension %d (32, 64 or 128)", who, dim);
+  IRX_REQUIRE(P.batch >= 0 && P.tq >= 0 && P.tk >= 0, "%s: negative size", who);
+  IRX_REQUIRE(P.heads >= 1 && P.kv_heads >= 1 && P.heads % P.kv_heads == 0, "%s: %d heads over %d key / value heads", who, P.heads, P.kv_heads);
+  IRX_REQUIRE(P.scale > 0.f && P.scale <= 3.402823466e38f, "%s: the scale must be positive and finite", who);
+  IRX_REQUIRE(P.cu_q && P.cu_k, "%s: null offsets", who);
+  const AtTensor* ts[4] = {&P.q, &P.k, &P.v, &P.dout};
+  for (int i = 0; i < 4; ++i) {
+    const AtTensor& t = *ts[i];
+    if (i == 3 && !t.p) continue;
+    const int rows = (i == 0 || i == 3) ? P.tq : P.tk;
+    IRX_REQUIRE(t.p || rows == 0, "%s: null tensor", who);
+    IRX_REQUIRE(((uintptr_t)t.p & 15) == 0 && (t.st * elem) % 16 == 0 && (t.sh * elem) % 16 == 0, "%s: rows and heads must start on 16 bytes", who);
+    IRX_REQUIRE(t.st >= 0 && t.sh >= 0, "%s: negative stride", who);
+  }
+  if (P.table) {
+    IRX_REQUIRE(P.map && P.buckets >= 1, "%s: a bias table needs its bucket map", who);
+    IRX_REQUIRE(P.far >= 0 && P.far <= IRX_ATTN_MAX_FAR, "%s: clipped distance %d (at most %d)", who, P.far, IRX_ATTN_MAX_FAR);
+  }
+  const long long rows = P.tq > P.tk ? P.tq : P.tk;
+  IRX_REQUIRE(rows + P.batch + 2 < (1ll << 30), "%s: too many rows", who);
+  IRX_REQUIRE((rows / IRX_ATTN_BM + P.batch + 2) * P.heads < (1ll << 25), "%s: too many tiles", who);
+  return IRX_OK;
+}
+
+// Parts of the key axis: one, unless the whole launch is far below one workgroup per compute unit and there are many keys per sequence.
+static int fwd_splits(long long tq, long long tk, int batch, int heads) {
+  if (batch <= 0 || tk <= 0) return 1;
+  const long long wgs = (tq / IRX_ATTN_BM + (batch < tq ? batch : tq)) * heads, keys = tk / batch;
+  if (wgs >= 512 || keys < 1024) return 1;
+  long long s = 1024 / (wgs > 0 ? wgs : 1);
+  if (s > keys / 256) s = keys / 256;
+  return s < 1 ? 1 : s > 32 ? 32 : (int)s;
+}
+
+extern "C" size_t irx_attn_packed_fwd_workspace_bytes(int tq, int tk, int batch, int heads, int dim) {
+  if (tq <= 0 || tk < 0 || batch < 0 || heads <= 0 || dim <= 0) return 0;
+  const int s = fwd_splits(tq, tk, batch, heads);
+  return s <= 1 ? 0 : (size_t)s * heads * tq * (dim + 2) * sizeof(float);
+}
+
+extern "C" int irx_attn_packed_fwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
+                                   const void* v, long long v_row, long long v_head, const int32_t* cu_q, const int32_t* cu_k, int batch,
+                                   int tq, int tk, int heads, int kv_heads, int dim, int dtype, float scale, int causal, const void* table,
+                                   int table_f32, const int32_t* map, int buckets, int far, void* out, float* stats, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  AtParams P = {};
+  P.q = {q, q_row, q_head};
+  P.k = {k, k_row, k_head};
+  P.v = {v, v_row, v_head};
+  P.cu_q = cu_q; P.cu_k = cu_k;
+  P.batch = batch; P.tq = tq; P.tk = tk; P.heads = heads; P.kv_heads = kv_heads; P.causal = causal != 0; P.scale = scale;
+  P.table = table; P.table_f32 = table_f32; P.map = map; P.buckets = buckets; P.far = far;
+  P.dst = out; P.wstats = stats;
+  if (int rc = at_check("irx_attn_packed_fwd", P, dim, dtype, dtype == IRX_ATTN_F32 ? 4 : 2)) return rc;
+  if (tq == 0) return IRX_OK;
+  IRX_REQUIRE(out && ((uintptr_t)out & 15) == 0, "irx_attn_packed_fwd: out must be given and start on 16 bytes");
+  P.slots = at_slots(tq, batch, IRX_ATTN_BM);
+  P.splits = fwd_splits(tq, tk, batch, heads);
+  if (P.splits > 1) {
+    const size_t need = irx_attn_packed_fwd_workspace_bytes(tq, tk, batch, heads, dim);
+    if (!workspace || workspace_bytes < need) {
+      irx_set_error("irx_attn_packed_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+      return IRX_ERR_WORKSPACE;
+    }
+    IRX_REQUIRE(((uintptr_t)workspace & 15) == 0, "irx_attn_packed_fwd: workspace must start on 16 bytes");
+    P.so = static_cast<float*>(workspace);
+    P.sst = P.so + (size_t)P.splits * heads * tq * dim;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == IRX_ATTN_F32) return launch_fwd_d<AtF32>(P, dim, st);
+  if (dtype == IRX_ATTN_BF16) return launch_fwd_d<AtBf16>(P, dim, st);
+  return launch_fwd_d<AtF16>(P, dim, st);
+}

@@ -470,6 +470,7 @@ void bind(const std::unordered_map<std::string, uint64_t>& addr) {
 namespace irxn {
 last_error_fn g_last_error = nullptr;
 void register_heads(pybind11::module& m);      // heads_nodes.cpp
+void register_text(pybind11::module& m);       // text_nodes.cpp
 }  // namespace irxn
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -483,4 +484,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("backward_tables", &backward_tables);
   m.def("kmaps_build_pyramid", &kmaps_build_pyramid);
   irxn::register_heads(m);
+  irxn::register_text(m);
 }

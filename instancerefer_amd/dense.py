@@ -463,3 +463,89 @@ def mlp2(seq, x, seed=None):
                             momentum, drop_p, seed if seed < (1 << 63) else seed - (1 << 64), _lib.stream_ptr(), slots, keep)
     return MLP2Fn.apply(x, lin1.weight, lin1.bias, nrm.weight, nrm.bias, lin2.weight, lin2.bias, norm, nrm.eps, rmean, rvar,
                         momentum, drop_p, seed)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# Root-mean-square norm with the residual's addition (csrc/irx_rmsnorm.hip)
+_NORM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _rms_forward(x2, r2, weight, eps, want_rstd):
+    rows, cols = x2.shape
+    y = torch.empty_like(x2)
+    h = torch.empty_like(x2) if r2 is not None else None
+    rstd = torch.empty(rows, dtype=_f32, device=x2.device) if want_rstd else None
+    _lib.call("irx_rms_norm_fwd", x2.data_ptr(), r2.data_ptr() if r2 is not None else None, weight.data_ptr(),
+              1 if weight.dtype == _f32 else 0, rows, cols, _NORM_TYPES[x2.dtype], eps, y.data_ptr(),
+              h.data_ptr() if h is not None else None, rstd.data_ptr() if want_rstd else None, _lib.stream_ptr())
+    return y, h, rstd
+
+
+class RMSNormFn(torch.autograd.Function):
+    """irx_rms_norm_fwd / irx_rms_norm_bwd as one node: (x, residual | None, weight) -> (y, h) or y alone without a residual."""
+
+    @staticmethod
+    def forward(ctx, x2, r2, weight, eps):
+        y, h, rstd = _rms_forward(x2, r2, weight, eps, True)
+        ctx.save_for_backward(x2 if h is None else h, weight, rstd)
+        ctx.set_materialize_grads(False)
+        return y if h is None else (y, h)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight, rstd = ctx.saved_tensors
+        rows, cols = h.shape
+        if dy is None and dh is None:
+            return None, None, None, None
+        if torch.cuda.is_current_stream_capturing():
+            from . import _nodes
+            _nodes.refuse_foreign_leaves("rms_norm_residual", _nodes.leaves_of(ctx))
+        dy = torch.zeros_like(h) if dy is None else dy.contiguous()
+        dh = None if dh is None else dh.contiguous()
+        dx = torch.empty_like(h)
+        dw = torch.empty_like(weight)
+        n = int(_lib.load().irx_rms_norm_bwd_workspace_bytes(rows, cols, _NORM_TYPES[h.dtype]))
+        ws = torch.empty(n, dtype=torch.uint8, device=h.device)
+        _lib.call("irx_rms_norm_bwd", dy.data_ptr(), dh.data_ptr() if dh is not None else None, h.data_ptr(), weight.data_ptr(),
+                  1 if weight.dtype == _f32 else 0, rstd.data_ptr(), rows, cols, _NORM_TYPES[h.dtype], dx.data_ptr(), dw.data_ptr(),
+                  ws.data_ptr(), n, _lib.stream_ptr())
+        return dx, dx if ctx.needs_input_grad[1] else None, dw, None
+
+
+def rms_norm_residual(x, residual, weight, eps=1e-6):
+    """(y, h): h = x + residual rounded to x's type, y = h / sqrt(mean(h^2 over the last axis) + eps) * weight — the step between two blocks
+    of a pre-norm encoder in one launch each way: h is the new residual stream, y goes into the next block. residual None: h is x.
+
+    x, residual (..., C) float32, bfloat16 or float16; weight (C,) float32 or x's type. Differentiable in all three (once); the gradient
+    with respect to h (what the later blocks send back) joins the norm's in the same launch."""
+    if x.dim() < 1 or x.shape[-1] < 1 or x.dtype not in _NORM_TYPES:
+        raise ValueError("rms_norm_residual: x must be (..., C) in float32, bfloat16 or float16, got %s of %s" % (tuple(x.shape), x.dtype))
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError("rms_norm_residual: x is %s of %s, the residual %s of %s" % (tuple(x.shape), x.dtype, tuple(residual.shape), residual.dtype))
+    if weight.shape != x.shape[-1:] or weight.dtype not in (_f32, x.dtype):
+        raise ValueError("rms_norm_residual: weight must be (%d,) in float32 or %s, got %s of %s" % (x.shape[-1], x.dtype, tuple(weight.shape), weight.dtype))
+    eps = float(eps)
+    if not 0.0 <= eps < math.inf:
+        raise ValueError("rms_norm_residual: eps must be >= 0 and finite, got %r" % eps)
+    for t in (x, residual, weight):
+        if t is not None and not t.is_cuda:
+            raise RuntimeError("irx operators need tensors on a HIP device (got %s); the CPU path exists only as the test oracle under /oracle" % t.device)
+        if t is not None and t.device != x.device:
+            raise ValueError("rms_norm_residual: tensors on %s and %s" % (x.device, t.device))
+    if x.device.index != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return rms_norm_residual(x, residual, weight, eps)
+    shape = x.shape
+    x2 = x.contiguous().view(-1, shape[-1])
+    r2 = None if residual is None else residual.contiguous().view(-1, shape[-1])
+    weight = weight.contiguous()
+    if torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad or (r2 is not None and r2.requires_grad)):
+        if torch.cuda.is_current_stream_capturing():
+            from . import _nodes
+            _nodes.refuse_foreign_leaves("rms_norm_residual", (x2, r2, weight))
+        out = RMSNormFn.apply(x2, r2, weight, eps)
+        y, h = (out, None) if r2 is None else out
+    else:
+        y, h, _ = _rms_forward(x2, r2, weight, eps, False)
+    return y.view(shape), x if h is None else h.view(shape)

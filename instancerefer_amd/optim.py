@@ -18,6 +18,9 @@ gather instead, so the sequence of collectives never depends on the data.
 
 Buffer management, gather, all-reduce, broadcast and the state dict work on any device (the world-size-2 gloo test
 runs them on CPU tensors); `step()` is the HIP kernel and raises without a HIP device — there is no CPU optimizer."""
+import ctypes
+import math
+
 import numpy as np
 import torch
 import torch.distributed as dist
@@ -50,6 +53,66 @@ def broadcast_buffers(module, src=0):
             for b in group:
                 b.copy_(flat[off:off + b.numel()].view_as(b))
                 off += b.numel()
+
+
+_CLIP_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _clip_args(who, max_norm, norm_type):
+    max_norm, norm_type = float(max_norm), float(norm_type)
+    if not max_norm >= 0.0:
+        raise ValueError("%s: max_norm must be >= 0, got %r" % (who, max_norm))
+    if norm_type not in (2.0, math.inf):
+        raise ValueError("%s: norm_type must be 2 or inf, got %r" % (who, norm_type))
+    return max_norm, int(norm_type == math.inf)
+
+
+@torch.no_grad()
+def clip_grads_(grads, max_norm, norm_type=2.0):
+    """Clip the GLOBAL norm of a list of gradients to max_norm, in place (csrc/irx_optim.hip): every value is multiplied by
+    min(1, max_norm / (norm + 1e-6)). Returns the norm before clipping as a 0-dim float32 tensor on their device (no host read; NaN or
+    infinite where the gradients are, and a NaN norm makes every gradient NaN). For parameters held by FlatAdam use its
+    backward_step(max_norm=...): no pass of its own over the gradients.
+
+    grads: dense float32, bfloat16 or float16 tensors on one device, mixed freely; None entries are skipped. No two may share memory.
+    norm_type: 2 or inf."""
+    max_norm, inf_norm = _clip_args("clip_grads_", max_norm, norm_type)
+    grads = [grads] if isinstance(grads, torch.Tensor) else [g for g in grads if g is not None]
+    if not grads:
+        return torch.zeros(())
+    dev, back, flat = grads[0].device, [], []
+    for g in grads:
+        if g.layout != torch.strided or g.dtype not in _CLIP_TYPES:
+            raise ValueError("clip_grads_: dense float32, bfloat16 or float16 tensors, got %s of %s" % (g.layout, g.dtype))
+        if not g.is_cuda:
+            raise RuntimeError("irx operators need tensors on a HIP device (got %s); the CPU path exists only as the test oracle under /oracle" % g.device)
+        if g.device != dev:
+            raise ValueError("clip_grads_: tensors on %s and %s" % (dev, g.device))
+        if not (g.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(g)):      # any order of one gap-free range will do
+            if any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
+                raise ValueError("clip_grads_: an expanded tensor cannot be clipped in place")
+            c = g.contiguous()
+            back.append((g, c))
+            g = c
+        flat.append(g)
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _clip(flat, back, max_norm, inf_norm)
+    return _clip(flat, back, max_norm, inf_norm)
+
+
+def _clip(flat, back, max_norm, inf_norm):
+    n = len(flat)
+    ptrs = (ctypes.c_void_p * n)(*[g.data_ptr() for g in flat])
+    types = (ctypes.c_int * n)(*[_CLIP_TYPES[g.dtype] for g in flat])
+    counts = (ctypes.c_ulonglong * n)(*[g.numel() for g in flat])
+    nb = int(_lib.load().irx_clip_grads_workspace_bytes(counts, n))
+    ws = torch.empty(nb, dtype=torch.uint8, device=flat[0].device)
+    norm = torch.empty((), dtype=torch.float32, device=flat[0].device)
+    _lib.call("irx_clip_grads", ptrs, types, counts, n, inf_norm, max_norm, norm.data_ptr(), ws.data_ptr(), nb, _lib.stream_ptr())
+    for g, c in back:
+        g.copy_(c)
+    return norm
 
 
 # Liveness of an optimizer's native gradient sink: a cell in the optimizer's own record tensor (row 256), 1 while this optimizer owns
@@ -370,18 +433,37 @@ class FlatAdam:
             self._runs_cache[key] = runs
         return runs
 
-    def step(self):
+    def step(self, max_norm=None, norm_type=2.0):
+        """Adam on the gathered gradients. max_norm: the gradients' global norm (over every parameter, of the gradients averaged over
+        the ranks; norm_type 2 or inf) is clipped to it first — the factor goes into the Adam launch, flat_g stays as it is. Returns the norm
+        before clipping as a 0-dim device tensor (no host read), or None without max_norm."""
+        if max_norm is not None:
+            return self._step_clipped(*_clip_args("FlatAdam.step", max_norm, norm_type))
         for lo, hi, step in self._runs():
             _lib.call("irx_adam_step", _lib.ptr(self.flat_p[lo:hi]), _lib.ptr(self.flat_g[lo:hi]),
                       _lib.ptr(self.exp_avg[lo:hi]), _lib.ptr(self.exp_avg_sq[lo:hi]), hi - lo, float(self.lr),
                       float(self.betas[0]), float(self.betas[1]), float(self.eps), float(self.weight_decay), step,
                       1.0 / self.world_size, _lib.stream_ptr())
 
-    def backward_step(self):
-        """After loss.backward(): gather -> all-reduce -> Adam."""
+    def _step_clipped(self, max_norm, inf_norm):
+        lib = _lib.load()
+        nb = int(lib.irx_grad_norm_workspace_bytes(self.n))
+        ws = torch.empty(nb, dtype=torch.uint8, device=self.device)
+        norm = torch.empty((), dtype=torch.float32, device=self.device)
+        _lib.call("irx_grad_norm_parts", _lib.ptr(self.flat_g), self.n, inf_norm, ws.data_ptr(), nb, _lib.stream_ptr())
+        runs = self._runs()
+        for lo, hi, step in runs:
+            _lib.call("irx_adam_step_clip", _lib.ptr(self.flat_p[lo:hi]), _lib.ptr(self.flat_g[lo:hi]),
+                      _lib.ptr(self.exp_avg[lo:hi]), _lib.ptr(self.exp_avg_sq[lo:hi]), hi - lo, float(self.lr),
+                      float(self.betas[0]), float(self.betas[1]), float(self.eps), float(self.weight_decay), step,
+                      1.0 / self.world_size, ws.data_ptr(), self.n, inf_norm, max_norm, norm.data_ptr(), _lib.stream_ptr())
+        return norm if runs else norm.zero_()           # (no parameter had a gradient)
+
+    def backward_step(self, max_norm=None, norm_type=2.0):
+        """After loss.backward(): gather -> all-reduce -> (clip ->) Adam. Returns what step() returns."""
         self.gather_grads()
         self.all_reduce()
-        self.step()
+        return self.step(max_norm, norm_type)
 
     # ---- torch.optim.Adam-compatible state (reference scripts/train.py:114-119 calls optimizer.load_state_dict) ----
     def state_dict(self):

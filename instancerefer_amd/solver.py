@@ -68,12 +68,13 @@ def resume_base_lr(saved_lr, initial_lr, start_epoch, lr_decay_step, lr_decay_ra
 
 class Solver:
     def __init__(self, model, config, dataloader, lr=1e-3, weight_decay=1e-5, lr_decay_step=(15, 20), lr_decay_rate=0.1,
-                 out_dir=None, verbose=20, device=None, use_checkpoint=None, sync_bn=False):
+                 out_dir=None, verbose=20, device=None, use_checkpoint=None, sync_bn=False, max_grad_norm=None):
         if not torch.cuda.is_initialized():        # the queue count is read once, when the HIP runtime starts (configure_hw_queues)
             from . import configure_hw_queues
             configure_hw_queues()
         self.device = device or torch.device("cuda", torch.cuda.current_device())
         self.model = model.to(self.device)
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)   # None: no clipping, as the reference
         self.sync_bn = bool(sync_bn)
         self.sync_bn_skipped = 0                   # steps dropped by sync_bn_guard (same count on every rank)
         if sync_bn:                                # world > 1: BatchNorm statistics over all ranks (syncbn.py)
@@ -198,7 +199,7 @@ class Solver:
             if one is None or one.device != loss.device or one.shape != loss.shape or one.dtype != loss.dtype:
                 one = self.__dict__["_unit_grad"] = torch.ones_like(loss)
             loss.backward(gradient=one)
-            self.optimizer.backward_step()
+            grad_norm = self.optimizer.backward_step(max_norm=self.max_grad_norm)      # a device scalar, or None without clipping
             self.global_iter += 1
             seen += data_dict["lang_scores"].shape[0]
             if self.global_iter % self.verbose == 0:
@@ -212,6 +213,8 @@ class Solver:
                            lang_acc=float(ev["lang_acc"]), ref_acc=float(np.mean(ev["ref_acc"])),
                            iou_rate_25=ev["ref_iou_rate_0.25"], iou_rate_5=ev["ref_iou_rate_0.5"],
                            scenes_per_sec=self.world * seen / dt)
+                if grad_norm is not None:
+                    rec["grad_norm"] = float(grad_norm)
                 rec["seg_acc"] = float(data_dict["seg_acc"].detach()) if "seg_acc" in data_dict else None
                 self.log["train"].append(rec)
                 self._scalars("train", rec)

@@ -1,0 +1,120 @@
+"""The operators of a text encoder's block as they are used together: norm + residual, attention over packed descriptions with a position
+bias, backward through both, clipping and the optimizer's step."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+class Block(torch.nn.Module):
+    def __init__(self, width=64, heads=4, kv=2, buckets=16):
+        super().__init__()
+        self.heads, self.kv, self.dim = heads, kv, width // heads
+        self.n1, self.n2 = torch.nn.Parameter(torch.ones(width)), torch.nn.Parameter(torch.ones(width))
+        self.qkv = torch.nn.Linear(width, (heads + 2 * kv) * self.dim, bias=False)
+        self.out = torch.nn.Linear(width, width, bias=False)
+        self.up, self.down = torch.nn.Linear(width, 2 * width), torch.nn.Linear(2 * width, width)
+        self.table = torch.nn.Parameter(torch.zeros(buckets, heads))
+
+    def forward(self, x, stream, cu, buckets, plain=False):
+        norm = plain_norm if plain else __import__("instancerefer_amd.dense", fromlist=["x"]).rms_norm_residual
+        a, stream = norm(x, stream, self.n1)
+        h, k, d = self.heads, self.kv, self.dim
+        f = self.qkv(a)
+        q, kk, v = f[:, :h * d].view(-1, h, d), f[:, h * d:(h + k) * d].view(-1, k, d), f[:, (h + k) * d:].view(-1, k, d)
+        if plain:
+            o = plain_attention(q, kk, v, cu, self.table, buckets)
+        else:
+            from instancerefer_amd.attention import attention_packed
+            o = attention_packed(q, kk, v, cu, bias=self.table, buckets=buckets)
+        b, stream = norm(self.out(o.reshape(-1, h * d)), stream, self.n2)
+        return self.down(torch.relu(self.up(b))), stream
+
+
+def plain_norm(x, r, w):
+    h = x + r
+    return h * torch.rsqrt(h.square().mean(-1, keepdim=True) + 1e-6) * w, h
+
+
+def plain_attention(q, k, v, cu, table, buckets):
+    outs, far = [], (buckets.shape[0] - 1) // 2
+    for b in range(cu.shape[0] - 1):
+        s = slice(int(cu[b]), int(cu[b + 1]))
+        n = int(cu[b + 1] - cu[b])
+        rel = torch.arange(n, device=q.device)[None, :] - torch.arange(n, device=q.device)[:, None]
+        g = q.shape[1] // k.shape[1]
+        kk, vv = k[s].repeat_interleave(g, 1), v[s].repeat_interleave(g, 1)
+        score = torch.matmul(q[s].transpose(0, 1), kk.permute(1, 2, 0)) / math.sqrt(q.shape[2])
+        score = score + table[buckets.long()[rel.clamp(-far, far) + far]].permute(2, 0, 1)
+        outs.append(torch.matmul(torch.softmax(score, -1), vv.transpose(0, 1)).transpose(0, 1))
+    return torch.cat(outs)
+
+
+def build(seed):
+    torch.manual_seed(seed)
+    blocks = torch.nn.ModuleList([Block(), Block()])
+    with torch.no_grad():
+        for b in blocks:
+            b.table.normal_()
+    return blocks
+
+
+def test_two_blocks_train_like_the_plain_formulas():
+    from instancerefer_amd.attention import packed_offsets, relative_buckets
+    from instancerefer_amd.optim import FlatAdam
+    lens = torch.tensor([11, 1, 40, 0, 126, 30])
+    rows = int(lens.sum())
+    g = torch.Generator().manual_seed(1)
+    words, target = torch.randn(rows, 64, generator=g), torch.randn(rows, 64, generator=g)
+    ref = build(3).double()
+    ours = build(3).to(DEV)
+    opt = FlatAdam(ours.parameters(), lr=1e-3)
+    cu, buckets = packed_offsets(lens.to(DEV)), relative_buckets(16, 60, device=DEV)
+
+    def loss_of(blocks, x, t, cu, buckets, plain):
+        stream = torch.zeros_like(x)
+        for b in blocks:
+            x, stream = b(x, stream, cu, buckets, plain)
+        return ((x + stream - t) ** 2).mean()
+
+    for step in range(3):
+        # the reference takes over the weights before every step: one step is compared, not a trajectory
+        with torch.no_grad():
+            for p, r in zip(ours.parameters(), ref.parameters()):
+                r.copy_(p.double().cpu())
+        want = loss_of(ref, words.double(), target.double(), cu.cpu(), buckets.cpu(), True)
+        grads = torch.autograd.grad(want, list(ref.parameters()))
+        opt.zero_grad()
+        loss = loss_of(ours, words.to(DEV), target.to(DEV), cu, buckets, False)
+        loss.backward()
+        assert abs(float(loss.detach()) - float(want)) <= 1e-5 * float(want)
+        for p, w in zip(ours.parameters(), grads):
+            # 32-bit arithmetic through two blocks: sums of up to 208 rows and 128 columns, some twenty operations deep
+            assert float((p.grad.double().cpu() - w).norm()) <= 2e-5 * float(w.norm()) + 1e-9
+        norm = math.sqrt(sum(float(w.square().sum()) for w in grads))
+        got = opt.backward_step(max_norm=0.5 * norm)
+        assert abs(float(got) - norm) <= 2e-5 * norm
+        # m / sqrt(v) of the first moments: the factor is in both, so compare the first moment itself
+        if step == 0:
+            first = torch.cat([(0.1 * 0.5 * w).reshape(-1) for w in grads])
+            have = torch.cat([opt.exp_avg[o:o + p.numel()].double().cpu() for p, o in zip(opt.params, opt.offsets)])
+            assert float((have - first).norm()) <= 4e-5 * float(first.norm())
+
+
+def test_solver_clips():
+    from instancerefer_amd import synthetic as S
+    from instancerefer_amd.instancerefer import InstanceRefer
+    from instancerefer_amd.loss_helper import DatasetConfig
+    from instancerefer_amd.solver import Solver, SyntheticLoader
+    kw = dict(num_points=3000, num_instances=5, num_candidates=[3, 2], tokens=[20, 9], points_per_instance=128)
+    model = InstanceRefer(7, S.default_args())
+    solver = Solver(model, DatasetConfig(), {"train": SyntheticLoader(2, 2, **kw)}, verbose=1, max_grad_norm=0.05)
+    solver.train_epoch(0)
+    assert len(solver.log["train"]) == 2
+    for rec in solver.log["train"]:
+        assert math.isfinite(rec["grad_norm"]) and rec["grad_norm"] > 0.05
+    # the first moment after one step is (1 - beta1) times a gradient of norm at most 0.05 (+ the weight decay's 1e-5 |p|)
+    assert float(solver.optimizer.exp_avg.norm()) <= 0.1 * (0.05 * 2 + 1e-5 * 2 * float(solver.optimizer.flat_p.norm())) * 1.01
