@@ -409,6 +409,8 @@ enum {
 /* Stream `to` continues behind everything enqueued on stream `from` so far (event record + wait; the library owns the events).
  * For callers that issue independent halves of one operator on two streams — plumbing, no reference counterpart. */
 int irx_stream_fork(void* from, void* to);
+/* 1 while `stream` is being captured into a graph, 0 otherwise (also for the null stream, which cannot be). Host call. */
+int irx_stream_capturing(void* stream);
 
 /* Launch order of the 64-row output tiles of a stride-1 convolution over table `nbr` (int32 [K][ld], the irx_kmap_build_s1
  * table): order[i] = i-th tile to start, heaviest cost class first (cost = per active offset a fixed part + one part per

@@ -19,6 +19,9 @@ _HEAD_ENTRY_POINTS = ("irx_mlp2_saved_floats", "irx_mlp2_fwd", "irx_mlp2_bwd", "
                       "irx_spconv_wgrad_workspace_bytes", "irx_spconv_wgrad", "irx_bn_workspace_bytes", "irx_bn_forward", "irx_bn_backward",
                       "irx_kmap_down_transpose", "irx_attn_pool_fwd", "irx_attn_pool_bwd", "irx_dropout_flat", "irx_stream_fork", "irx_total_loss", "irx_edgeconv_workspace_bytes",
                       "irx_edgeconv_max_fwd", "irx_edgeconv_max_bwd", "irx_lang_pool_fwd", "irx_lang_pool_bwd")
+# csrc/text_nodes.cpp (packed attention, norm with residual)
+_TEXT_ENTRY_POINTS = ("irx_attn_packed_fwd_workspace_bytes", "irx_attn_packed_fwd", "irx_attn_packed_bwd_workspace_bytes", "irx_attn_packed_bwd",
+                      "irx_rms_norm_fwd", "irx_rms_norm_bwd_workspace_bytes", "irx_rms_norm_bwd", "irx_stream_capturing", "irx_last_error")
 _mod = None
 _tried = False
 _lock = __import__("threading").Lock()
@@ -55,6 +58,7 @@ def _load_locked():
         lib = _lib.load()
         mod.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _ENTRY_POINTS})
         mod.bind_heads({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _HEAD_ENTRY_POINTS})
+        mod.bind_text({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _TEXT_ENTRY_POINTS})
     except Exception as e:                 # a module built against another torch: say so, run the heads through their Python nodes
         import warnings
         warnings.warn("instancerefer_amd: csrc/_irx_nodes.so could not be loaded (%s: %s) — the dense heads run through their "

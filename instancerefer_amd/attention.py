@@ -21,6 +21,7 @@ can reach earlier rows of its tile of 64 under `causal`, as in any matrix produc
 next of them (a copy), up to 128. Deterministic; captures into a graph (the offsets may change between replays, the shapes may not). A capture with gradients is refused
 while an eager graph of the same leaves lives on another stream."""
 import math
+import os
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -30,6 +31,7 @@ from . import _lib, _nodes
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _DIMS = (32, 64, 128)
 MAX_FAR = 512
+BACKEND = os.environ.get("IRX_ATTENTION_BACKEND", "auto")   # "py": the Python autograd.Function below even when the C++ node exists
 
 
 def packed_offsets(lengths):
@@ -198,6 +200,9 @@ def attention_packed(q, k, v, cu_q, cu_k=None, causal=False, scale=None, bias=No
         more = next(d for d in _DIMS if d > dim) - dim
         q, k, v = (torch.nn.functional.pad(t, (0, more)) for t in (q, k, v))
         return attention_packed(q, k, v, cu_q, cu_k, causal, scale, bias, buckets)[..., :dim]
+    nodes = _nodes.load() if BACKEND != "py" else None
+    if nodes is not None:
+        return nodes.attention(q, k, v, bias, cu_q, cu_k, buckets, bool(causal), scale, _lib.stream_ptr())
     q, k, v = _rows(q), _rows(k), _rows(v)
     if bias is not None:
         bias = bias.contiguous()

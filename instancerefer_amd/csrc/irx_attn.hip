@@ -300,3 +300,13 @@ extern "C" int irx_attn_packed_fwd(const void* q, long long q_row, long long q_h
   if (dtype == IRX_ATTN_BF16) return launch_fwd_d<AtBf16>(P, dim, st);
   return launch_fwd_d<AtF16>(P, dim, st);
 }
+
+extern "C" int irx_stream_capturing(void* stream) {
+  if (!stream) return 0;
+  hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing((hipStream_t)stream, &s) != hipSuccess) {
+    (void)hipGetLastError();
+    return 0;
+  }
+  return s != hipStreamCaptureStatusNone;
+}

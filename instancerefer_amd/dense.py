@@ -467,6 +467,7 @@ def mlp2(seq, x, seed=None):
 
 # ---------------------------------------------------------------------------------------------------------------------
 # Root-mean-square norm with the residual's addition (csrc/irx_rmsnorm.hip)
+NORM_BACKEND = os.environ.get("IRX_NORM_BACKEND", "auto")   # "py": the Python autograd.Function below even when the C++ node exists
 _NORM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -540,6 +541,12 @@ def rms_norm_residual(x, residual, weight, eps=1e-6):
     x2 = x.contiguous().view(-1, shape[-1])
     r2 = None if residual is None else residual.contiguous().view(-1, shape[-1])
     weight = weight.contiguous()
+    if NORM_BACKEND != "py":
+        from . import _nodes
+        nodes = _nodes.load()
+        if nodes is not None:
+            out = nodes.rms_norm(x2, r2, weight, eps, _lib.stream_ptr())
+            return out[0].view(shape), x if r2 is None else out[1].view(shape)
     if torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad or (r2 is not None and r2.requires_grad)):
         if torch.cuda.is_current_stream_capturing():
             from . import _nodes

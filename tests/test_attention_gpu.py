@@ -8,6 +8,17 @@ from attention_ref import check, reference
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+
+
+@pytest.fixture(params=["cpp", "py"])
+def backend(request, monkeypatch):
+    """the C++ autograd node and the Python one"""
+    from instancerefer_amd import attention, _nodes
+    if request.param == "cpp":
+        assert _nodes.load() is not None
+    monkeypatch.setattr(attention, "BACKEND", "py" if request.param == "py" else "auto")
+
+
 TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 
 
@@ -75,7 +86,7 @@ def test_position_bias_and_its_gradient(kind, both, narrow):
     compare([1, 40, 150, 333], [1, 40, 150, 333], 4, 2, 64, kind, not both, table=table, buckets=relative_buckets(16, 50, both), seed=7)
 
 
-def test_position_bias_with_keys_of_their_own_length_and_a_free_map():
+def test_position_bias_with_keys_of_their_own_length_and_a_free_map(backend):
     table = torch.randn(5, 2, generator=torch.Generator().manual_seed(1))
     buckets = torch.randint(0, 5, (2 * 512 + 1,), generator=torch.Generator().manual_seed(2), dtype=torch.int32)
     compare([90, 7, 1], [33, 700, 0], 2, 2, 32, "f32", False, table=table, buckets=buckets)
@@ -133,7 +144,7 @@ def test_infinite_keys_behind_the_causal_border_do_not_matter():
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
-def test_strided_views_and_other_head_dimensions(kind):
+def test_strided_views_and_other_head_dimensions(kind, backend):
     from instancerefer_amd.attention import attention_packed
     dt, lens = TYPES[kind], [37, 100]
     g = torch.Generator().manual_seed(2)
@@ -239,7 +250,7 @@ def test_same_bits_every_time_and_on_another_stream():
             assert torch.equal(got[name], want[name]), name
 
 
-def test_captured_forward_and_backward_with_new_offsets():
+def test_captured_forward_and_backward_with_new_offsets(backend):
     from instancerefer_amd.attention import attention_packed, relative_buckets
     dt, total = torch.bfloat16, 260
     g = torch.Generator().manual_seed(6)
@@ -274,7 +285,7 @@ def test_captured_forward_and_backward_with_new_offsets():
             q.mul_(0.9)
 
 
-def test_capture_beside_a_living_eager_graph_is_refused():
+def test_capture_beside_a_living_eager_graph_is_refused(backend):
     """a captured backward would make the eager graph's stream wait inside the capture: refused before anything is recorded, in the forward
     and, where the forward was eager, in the backward"""
     from instancerefer_amd.attention import attention_packed
@@ -296,6 +307,16 @@ def test_capture_beside_a_living_eager_graph_is_refused():
     assert float(torch.autograd.grad(alive, q, do)[0].abs().max()) > 0
 
 
+def test_second_derivative_is_refused(backend):
+    from instancerefer_amd.attention import attention_packed
+    q, k, v, do = (t.to(DEV) for t in make([9], [9], 2, 2, 32, torch.float32, 71))
+    q.requires_grad_(True)
+    o = attention_packed(q, k, v, offsets([9]).to(DEV))
+    (dq,) = torch.autograd.grad((o * o).sum(), q, create_graph=True)      # a gradient that depends on q itself
+    with pytest.raises(RuntimeError, match="differentiable once|once_differentiable"):
+        dq.sum().backward()
+
+
 def test_offsets_are_clamped_to_the_rows():
     """offsets beyond the tensors reach no memory outside them: they are clamped on the device"""
     from instancerefer_amd.attention import attention_packed
@@ -305,7 +326,7 @@ def test_offsets_are_clamped_to_the_rows():
     assert torch.equal(got, want)
 
 
-def test_no_rows_and_no_keys():
+def test_no_rows_and_no_keys(backend):
     from instancerefer_amd.attention import attention_packed
     z = lambda n, h: torch.zeros(n, h, 64, device=DEV, requires_grad=True)  # noqa: E731
     cu0, cu = torch.zeros(1, dtype=torch.int32, device=DEV), torch.tensor([0, 0], dtype=torch.int32, device=DEV)

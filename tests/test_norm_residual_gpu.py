@@ -6,6 +6,17 @@ import torch
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+
+
+@pytest.fixture(params=["cpp", "py"])
+def backend(request, monkeypatch):
+    """the C++ autograd node and the Python one"""
+    from instancerefer_amd import dense, _nodes
+    if request.param == "cpp":
+        assert _nodes.load() is not None
+    monkeypatch.setattr(dense, "NORM_BACKEND", "py" if request.param == "py" else "auto")
+
+
 HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 U32 = 2.0 ** -24
 
@@ -74,7 +85,7 @@ def test_forward_and_gradients(kind, rows, cols, residual):
         assert torch.equal(y, y2) and torch.equal(s, s2)
 
 
-def test_one_output_used_alone():
+def test_one_output_used_alone(backend):
     from instancerefer_amd.dense import rms_norm_residual
     x, res, w, dy, dh = inputs(20, 96, torch.float32, torch.float32, 3)
     _, want = expected(x, res, w, dy, None, 1e-5)
@@ -84,7 +95,7 @@ def test_one_output_used_alone():
     assert torch.equal(torch.autograd.grad(h, xd, dh.to(DEV))[0].cpu(), dh)
 
 
-def test_shapes_strides_and_empty():
+def test_shapes_strides_and_empty(backend):
     from instancerefer_amd.dense import rms_norm_residual
     x, res, w, _, _ = inputs(12, 64, torch.bfloat16, torch.float32, 5)
     want = rms_norm_residual(x.to(DEV), res.to(DEV), w.to(DEV))
@@ -122,7 +133,7 @@ def test_against_differences():
         assert abs(want - have) <= 1e-2 * max(1.0, abs(have)), (n, want, have)       # third order: 1e-4; rounding of f: 1e-5 / 2e-2
 
 
-def test_captured_and_on_another_stream():
+def test_captured_and_on_another_stream(backend):
     from instancerefer_amd.dense import rms_norm_residual
     x, res, w, dy, dh = (t.to(DEV) for t in inputs(700, 512, torch.bfloat16, torch.float32, 9))
     for t in (x, res, w):
@@ -150,7 +161,7 @@ def test_captured_and_on_another_stream():
             x.mul_(1.1)
 
 
-def test_capture_beside_a_living_eager_graph_is_refused():
+def test_capture_beside_a_living_eager_graph_is_refused(backend):
     from instancerefer_amd.dense import rms_norm_residual
     x, res, w, dy, dh = (t.to(DEV) for t in inputs(7, 64, torch.float32, torch.float32, 10))
     w.requires_grad_(True)
