@@ -76,7 +76,7 @@ def relative_buckets(num_buckets, max_distance, bidirectional=True, device=None)
 def _rows(t):
     """The kernels read rows and heads in place from any strides that keep 16-byte alignment; everything else is copied."""
     e = t.element_size()
-    if t.stride(2) == 1 and t.stride(0) * e % 16 == 0 and t.stride(1) * e % 16 == 0 and t.data_ptr() % 16 == 0:
+    if t.stride(2) == 1 and t.stride(0) * e % 16 == 0 and t.stride(0) * e < 1 << 24 and t.stride(1) * e % 16 == 0 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)     # (contiguous() would keep a tensor that merely starts off 16 bytes)
 
@@ -131,7 +131,7 @@ class AttentionPackedFn(torch.autograd.Function):
         if table is not None:
             dt = torch.empty_like(table) if tq else torch.zeros_like(table)
         tb, tb_f32, mp, nb, far = _table_args(table, buckets)
-        n = int(_lib.load().irx_attn_packed_bwd_workspace_bytes(tq, batch, heads, far))
+        n = int(_lib.load().irx_attn_packed_bwd_workspace_bytes(tq, tk, batch, heads, kv_heads, dim, far))
         ws = torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
         _lib.call("irx_attn_packed_bwd", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
                   v.stride(0), v.stride(1), dout.data_ptr(), dout.stride(0), dout.stride(1), out.data_ptr(), stats.data_ptr(),

@@ -163,6 +163,32 @@ template <class T> __device__ __forceinline__ void at_st4(typename T::S* p, floa
   }
 }
 
+// ---- direct loads into LDS ----------------------------------------------------------------------------------------------------
+// In asm: with the builtin the compiler takes every later LDS read to depend on the load and waits where it was issued. The only wait is
+// at_landed() before the barrier that hands the tile over.
+typedef int at_i32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ at_i32x4 at_rsrc(const void* base, unsigned bytes) {
+  const unsigned long long b = (unsigned long long)base;
+  return (at_i32x4){__builtin_amdgcn_readfirstlane((int)(unsigned)b), __builtin_amdgcn_readfirstlane((int)((unsigned)(b >> 32) & 0xffffu)),
+                    __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
+}
+__device__ __forceinline__ unsigned at_lds_addr(const void* p) {
+  return (unsigned)(unsigned long long)(__attribute__((address_space(3))) const void*)p;
+}
+__device__ __forceinline__ void at_dma(at_i32x4 rs, unsigned lds, unsigned off) {
+  unsigned keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %2, %3, 0 offen lds\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "s"(lds), "v"(off), "s"(rs)
+      : "memory");
+}
+__device__ __forceinline__ void at_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // ---- LDS images -----------------------------------------------------------------------------------------------------------
 // A tile is BN rows of D elements, as they are in memory; the 16-byte pieces of a row are XOR-swizzled by the row so that neither reads
 // of one piece from 16 rows (ds_read_b128) nor transposing reads of 64 bytes from four rows meet in a bank (64 banks, 256 bytes a turn).
@@ -180,16 +206,24 @@ template <class T, int D> struct AtTile {
   }
   __device__ static __forceinline__ int at(int row, int piece) { return row * RB + ((piece ^ swz(row)) << 4); }
 
-  // rows first .. first + BN of a tensor (rows >= count: zeros) through registers into LDS
-  template <int THREADS> __device__ static __forceinline__ void copy_in(unsigned char* lds, const typename T::S* src, long long st, int count) {
-    constexpr int N = IRX_ATTN_BN * PIECES / THREADS;
+  // A tile's way into LDS: direct loads (16 bytes per lane, 1 KB per instruction, no registers in between). The LDS side is linear, so the
+  // swizzle is in the addresses: lane l of chunk c fills piece p of row r and asks for piece p ^ swz(r). Rows from `count` on lie behind
+  // the descriptor's end and arrive as zeros. The four waves take every fourth chunk.
+  enum { CHUNKS = BYTES / 4096 };
+  __device__ static __forceinline__ void dma_offsets(unsigned (&off)[CHUNKS], long long stride_bytes) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int id = i * THREADS + threadIdx.x, row = id / PIECES, piece = id % PIECES;
-      at_u32x4 v = {0u, 0u, 0u, 0u};
-      if (row < count) v = *reinterpret_cast<const at_u32x4*>(reinterpret_cast<const unsigned char*>(src + row * st) + piece * 16);
-      *reinterpret_cast<at_u32x4*>(lds + at(row, piece)) = v;
+    for (int i = 0; i < CHUNKS; ++i) {
+      const int byte = (4 * i + wave) * 1024 + lane * 16, row = byte / RB, piece = (byte % RB) / 16;
+      off[i] = (unsigned)row * (unsigned)stride_bytes + (unsigned)((piece ^ swz(row)) * 16);
     }
+  }
+  __device__ static __forceinline__ void dma(unsigned lds, const void* src, long long stride_bytes, int count, const unsigned (&off)[CHUNKS]) {
+    const unsigned n = count < IRX_ATTN_BN ? (unsigned)(count < 0 ? 0 : count) : IRX_ATTN_BN;
+    const at_i32x4 rs = at_rsrc(src, n ? (n - 1) * (unsigned)stride_bytes + RB : 0);
+    const unsigned at = lds + (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 1024;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) at_dma(rs, at + i * 4096, off[i]);
   }
   // A operand, rows row0 + l % 32, values 16 step + 8 (l / 32) .. + 7 of the row
   __device__ static __forceinline__ typename T::F row_frag(const unsigned char* lds, int row0, int step) {
@@ -229,7 +263,15 @@ template <class T, int D> struct AtTile {
   }
 };
 
-__device__ __forceinline__ float at_other_half(float x) { return __shfl_xor(x, 32, 64); }
+// the value of lane l ^ 32 joined with this lane's, without LDS (v_permlane32_swap)
+__device__ __forceinline__ float at_pair_max(float x) {
+  const at_u32x2 r = __builtin_bit_cast(at_u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float at_pair_sum(float x) {
+  const at_u32x2 r = __builtin_bit_cast(at_u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 __device__ __forceinline__ float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // dynamic LDS above the runtime's default of 64 KB has to be asked for

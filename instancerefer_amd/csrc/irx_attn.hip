@@ -15,9 +15,7 @@ __global__ __launch_bounds__(256, (T::ESZ == 4 && D == 128) ? 1 : 2) void k_attn
   typedef typename T::S S;
   constexpr int STEPS = D / 16, BLOCKS = D / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  unsigned char* lk_ = smem;
-  unsigned char* lv_ = smem + Tile::BYTES;
-  float* sb = reinterpret_cast<float*>(smem + 2 * Tile::BYTES);
+  float* sb = reinterpret_cast<float*>(smem + 4 * Tile::BYTES);           // two buffers of (keys, values) before it
 
   // consecutive workgroups go to the 8 XCDs in turn: give each XCD a contiguous run of (head, slot), so that a head's keys and values are
   // read through one L2; the last slots of a sequence, the longest ones under a causal mask, first
@@ -34,8 +32,8 @@ __global__ __launch_bounds__(256, (T::ESZ == 4 && D == 128) ? 1 : 2) void k_attn
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int kb = 0, ke = 0;
   if (sp.seq >= 0) {
-    kb = at_edge(P.cu_k, P.batch, P.tk, sp.seq + 1);
-    ke = at_edge(P.cu_k, P.batch, P.tk, sp.seq + 2);
+    kb = __builtin_amdgcn_readfirstlane(at_edge(P.cu_k, P.batch, P.tk, sp.seq + 1));
+    ke = __builtin_amdgcn_readfirstlane(at_edge(P.cu_k, P.batch, P.tk, sp.seq + 2));
   }
   const int lk = ke > kb ? ke - kb : 0, off = lk - (sp.end - first);
   const int row0 = sp.begin + wave * 32;
@@ -72,12 +70,26 @@ __global__ __launch_bounds__(256, (T::ESZ == 4 && D == 128) ? 1 : 2) void k_attn
     for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
   float m = -INFINITY, l = 0.f;               // l: this lane's half of the row only
 
+  // while a tile is worked on, the next one is on its way into the other buffer: one barrier per tile
+  const unsigned lds0 = at_lds_addr(smem);
+  const long long ks = P.k.st * T::ESZ, vs = P.v.st * T::ESZ;
+  unsigned ko[Tile::CHUNKS], vo[Tile::CHUNKS];
+  Tile::dma_offsets(ko, ks);
+  Tile::dma_offsets(vo, vs);
+  auto fetch = [&](int t) __attribute__((always_inline)) {
+    const unsigned to = lds0 + ((t - t0) & 1) * 2 * Tile::BYTES;
+    const int k0 = t * IRX_ATTN_BN;
+    Tile::dma(to, kp + k0 * P.k.st, ks, lk - k0, ko);
+    Tile::dma(to + Tile::BYTES, vp + k0 * P.v.st, vs, lk - k0, vo);
+  };
+  if (t0 < t1) fetch(t0);
   for (int t = t0; t < t1; ++t) {
     const int k0 = t * IRX_ATTN_BN;
+    at_landed();
     __syncthreads();
-    Tile::template copy_in<256>(lk_, kp + k0 * P.k.st, P.k.st, lk - k0);
-    Tile::template copy_in<256>(lv_, vp + k0 * P.v.st, P.v.st, lk - k0);
-    __syncthreads();
+    if (t + 1 < t1) fetch(t + 1);
+    const unsigned char* lk_ = smem + ((t - t0) & 1) * 2 * Tile::BYTES;
+    const unsigned char* lv_ = lk_ + Tile::BYTES;
     if (k0 >= wave_any) continue;
     float s[32];
 #pragma unroll
@@ -114,7 +126,7 @@ __global__ __launch_bounds__(256, (T::ESZ == 4 && D == 128) ? 1 : 2) void k_attn
     float mx = s[0];
 #pragma unroll
     for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i]);
-    mx = fmaxf(mx, at_other_half(mx));
+    mx = at_pair_max(mx);
     if constexpr (!BIAS) mx *= c1;                                       // c1 > 0
     // the running maximum moves only when a row outgrows it by 2^8: weights stay below 256, and most tiles rescale nothing
     if (__any(mx > m + 8.f || m == -INFINITY)) {
@@ -142,8 +154,8 @@ __global__ __launch_bounds__(256, (T::ESZ == 4 && D == 128) ? 1 : 2) void k_attn
       for (int b = 0; b < BLOCKS; ++b) acc[b] = at_mma(Tile::col_frag(lv_, 16 * ks, b), p, acc[b]);
     }
   }
+  l = at_pair_sum(l);
   if (!mine) return;
-  l += at_other_half(l);
   const float inv = l == 0.f ? 0.f : 1.f / l;                            // a row that sees nothing: zeros
   if (P.splits > 1) {
     const size_t r = ((size_t)part * P.heads + head) * P.tq + q;
@@ -205,7 +217,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AtParams P) {
 }
 
 template <class T, int D, bool BIAS> static int launch_fwd(const AtParams& P, hipStream_t st) {
-  const size_t lds = 2 * AtTile<T, D>::BYTES + (BIAS ? sizeof(float) * (2 * P.far + 1) : 0);
+  const size_t lds = 4 * AtTile<T, D>::BYTES + (BIAS ? sizeof(float) * (2 * P.far + 1) : 0);
   const long long total = (long long)P.slots * P.heads * P.splits;
   const unsigned grid = (unsigned)((total + 7) / 8 * 8);
   if (int rc = at_want_lds(reinterpret_cast<const void*>(&k_attn_fwd<T, D, BIAS>), lds, "irx_attn_packed_fwd")) return rc;
@@ -240,6 +252,7 @@ int at_check(const char* who, const AtParams& P, int dim, int dtype, int elem) {
     IRX_REQUIRE(t.p || rows == 0, "%s: null tensor", who);
     IRX_REQUIRE(((uintptr_t)t.p & 15) == 0 && (t.st * elem) % 16 == 0 && (t.sh * elem) % 16 == 0, "%s: rows and heads must start on 16 bytes", who);
     IRX_REQUIRE(t.st >= 0 && t.sh >= 0, "%s: negative stride", who);
+    IRX_REQUIRE(t.st * elem < (1ll << 24), "%s: rows more than 16 MB apart", who);      // 64 rows of a tile: 32-bit byte offsets
   }
   if (P.table) {
     IRX_REQUIRE(P.map && P.buckets >= 1, "%s: a bias table needs its bucket map", who);

@@ -25,9 +25,9 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
   typedef typename T::S S;
   constexpr int STEPS = D / 16, BLOCKS = D / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  unsigned char* lk_ = smem;
-  unsigned char* lv_ = smem + Tile::BYTES;
-  float* sb = reinterpret_cast<float*>(smem + 2 * Tile::BYTES);
+  // two buffers of (keys, values); one where two and the bias arrays do not fit the 160 KB
+  constexpr int BUFS = (T::ESZ == 4 && D == 128 && BIAS) ? 1 : 2;
+  float* sb = reinterpret_cast<float*>(smem + 2 * BUFS * Tile::BYTES);
   const int W = 2 * P.far + 1;
   float* sd = sb + W;                                                    // [wave][half][W]
 
@@ -47,8 +47,8 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int kb = 0, ke = 0;
   if (sp.seq >= 0) {
-    kb = at_edge(P.cu_k, P.batch, P.tk, sp.seq + 1);
-    ke = at_edge(P.cu_k, P.batch, P.tk, sp.seq + 2);
+    kb = __builtin_amdgcn_readfirstlane(at_edge(P.cu_k, P.batch, P.tk, sp.seq + 1));
+    ke = __builtin_amdgcn_readfirstlane(at_edge(P.cu_k, P.batch, P.tk, sp.seq + 2));
   }
   const int lk = ke > kb ? ke - kb : 0, off = lk - (sp.end - first);
   const int row0 = sp.begin + wave * 32;
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
 #pragma unroll
       for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(at_get<T>(of, e), at_get<T>(df[s], e), delta);
     }
-    delta += at_other_half(delta);
+    delta = at_pair_sum(delta);
     if (mine) {
       const float* st = P.stats + ((size_t)head * P.tq + q) * 2;
       m = st[0];
@@ -100,12 +100,25 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
 
+  const unsigned lds0 = at_lds_addr(smem);
+  const long long ks = P.k.st * T::ESZ, vs = P.v.st * T::ESZ;
+  unsigned ko[Tile::CHUNKS], vo[Tile::CHUNKS];
+  Tile::dma_offsets(ko, ks);
+  Tile::dma_offsets(vo, vs);
+  auto fetch = [&](int t) __attribute__((always_inline)) {
+    const unsigned to = lds0 + (t % BUFS) * 2 * Tile::BYTES;
+    const int k0 = t * IRX_ATTN_BN;
+    Tile::dma(to, kp + k0 * P.k.st, ks, lk - k0, ko);
+    Tile::dma(to + Tile::BYTES, vp + k0 * P.v.st, vs, lk - k0, vo);
+  };
+  if (t1 > 0) fetch(0);
   for (int t = 0; t < t1; ++t) {
     const int k0 = t * IRX_ATTN_BN;
+    at_landed();
     __syncthreads();
-    Tile::template copy_in<256>(lk_, kp + k0 * P.k.st, P.k.st, lk - k0);
-    Tile::template copy_in<256>(lv_, vp + k0 * P.v.st, P.v.st, lk - k0);
-    __syncthreads();
+    if (BUFS == 2 && t + 1 < t1) fetch(t + 1);
+    const unsigned char* lk_ = smem + (t % BUFS) * 2 * Tile::BYTES;
+    const unsigned char* lv_ = lk_ + Tile::BYTES;
 #pragma unroll
     for (int kb2 = 0; kb2 < 2; ++kb2) {
       const int k1 = k0 + 32 * kb2;
@@ -170,6 +183,10 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
         for (int b = 0; b < BLOCKS; ++b) acc[b] = at_mma(Tile::col_frag(lk_, 32 * kb2 + 16 * ks, b), f, acc[b]);
       }
     }
+    if (BUFS == 1) {
+      __syncthreads();
+      if (t + 1 < t1) fetch(t + 1);
+    }
   }
   if constexpr (BIAS) {
 #pragma unroll
@@ -211,17 +228,13 @@ __global__ __launch_bounds__(256, 1) void k_attn_dkv(AtParams P, int total) {
   // float16 keeps 10 bits below 2^-14: weights of long rows are that small, so they go through the product times 2^10
   constexpr float UP = T::ID == IRX_ATTN_F16 ? 1024.f : 1.f;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  unsigned char* lq_ = smem;
-  unsigned char* ld_ = smem + Tile::BYTES;
-  float* sm = reinterpret_cast<float*>(smem + 2 * Tile::BYTES);          // row maxima, 1 / row sums, D of the tile's 64 queries
-  float* si = sm + IRX_ATTN_BN;
-  float* se = si + IRX_ATTN_BN;
-  float* sb = se + IRX_ATTN_BN;
+  float* srow = reinterpret_cast<float*>(smem + 4 * Tile::BYTES);        // [buffer][row maxima | 1 / row sums | D][64 queries]
+  float* sb = srow + 6 * IRX_ATTN_BN;
 
   const int per = gridDim.x >> 3;
   const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if (id >= total) return;
-  const int slot = id % P.slots, kvh = id / P.slots;
+  const int slot = id % P.slots, rest = id / P.slots, kvh = rest % P.kv_heads, part = rest / P.kv_heads;
 
   int first;
   const AtSpan sp = at_span(P.cu_k, P.batch, P.tk, IRX_ATTN_BM, slot, &first);
@@ -230,8 +243,8 @@ __global__ __launch_bounds__(256, 1) void k_attn_dkv(AtParams P, int total) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int qb = 0, qe = 0;
   if (sp.seq >= 0) {
-    qb = at_edge(P.cu_q, P.batch, P.tq, sp.seq + 1);
-    qe = at_edge(P.cu_q, P.batch, P.tq, sp.seq + 2);
+    qb = __builtin_amdgcn_readfirstlane(at_edge(P.cu_q, P.batch, P.tq, sp.seq + 1));
+    qe = __builtin_amdgcn_readfirstlane(at_edge(P.cu_q, P.batch, P.tq, sp.seq + 2));
   }
   const int lq = qe > qb ? qe - qb : 0, off = (sp.end - first) - lq;
   const int row0 = sp.begin + wave * 32;
@@ -261,28 +274,56 @@ __global__ __launch_bounds__(256, 1) void k_attn_dkv(AtParams P, int total) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) dk[b][i] = dv[b][i] = 0.f;
 
-  for (int g = 0; g < group; ++g) {
-    const int head = kvh * group + g;
-    if constexpr (BIAS) {
-      __syncthreads();
-      at_load_bias<T>(sb, P, head);
-    }
-    const S* qp = reinterpret_cast<const S*>(P.q.p) + qb * P.q.st + head * P.q.sh;
-    const S* dp = reinterpret_cast<const S*>(P.dout.p) + qb * P.dout.st + head * P.dout.sh;
-    const float* st = P.stats + ((size_t)head * P.tq + qb) * 2;
-    const float* de = P.delta + (size_t)head * P.tq + qb;
-    for (int q0 = block_any / IRX_ATTN_BN * IRX_ATTN_BN; q0 < lq; q0 += IRX_ATTN_BN) {
-      __syncthreads();
-      Tile::template copy_in<256>(lq_, qp + q0 * P.q.st, P.q.st, lq - q0);
-      Tile::template copy_in<256>(ld_, dp + q0 * P.dout.st, P.dout.st, lq - q0);
-      if (threadIdx.x < IRX_ATTN_BN) {
-        const int r = q0 + (int)threadIdx.x;
-        const bool in = r < lq;
-        sm[threadIdx.x] = in ? st[2 * (size_t)r] : 0.f;
-        si[threadIdx.x] = in ? st[2 * (size_t)r + 1] : 0.f;
-        se[threadIdx.x] = in ? de[r] : 0.f;
+  // items (query head of the group, tile of 64 queries), in order; a launch with few workgroups gives each a part of them
+  const int tile0 = block_any / IRX_ATTN_BN, tiles = max((lq + IRX_ATTN_BN - 1) / IRX_ATTN_BN - tile0, 0);
+  const int it0 = (int)((long long)group * tiles * part / P.splits), it1 = (int)((long long)group * tiles * (part + 1) / P.splits);
+  const unsigned lds0 = at_lds_addr(smem);
+  const long long qs = P.q.st * T::ESZ, os = P.dout.st * T::ESZ;
+  unsigned qo[Tile::CHUNKS], oo[Tile::CHUNKS];
+  Tile::dma_offsets(qo, qs);
+  Tile::dma_offsets(oo, os);
+  float rm = 0.f, ri = 0.f, rd = 0.f;                                    // row statistics on their way (threads 0..63)
+  auto fetch = [&](int it) __attribute__((always_inline)) {
+    const int head = kvh * group + it / tiles, q0 = (tile0 + it % tiles) * IRX_ATTN_BN;
+    if (threadIdx.x < IRX_ATTN_BN) {
+      const int r = q0 + (int)threadIdx.x;
+      rm = ri = rd = 0.f;
+      if (r < lq) {
+        const size_t at = (size_t)head * P.tq + qb + r;
+        rm = P.stats[2 * at];
+        ri = P.stats[2 * at + 1];
+        rd = P.delta[at];
       }
-      __syncthreads();
+    }
+    const unsigned to = lds0 + ((it - it0) & 1) * 2 * Tile::BYTES;
+    Tile::dma(to, reinterpret_cast<const S*>(P.q.p) + (qb + q0) * P.q.st + head * P.q.sh, qs, lq - q0, qo);
+    Tile::dma(to + Tile::BYTES, reinterpret_cast<const S*>(P.dout.p) + (qb + q0) * P.dout.st + head * P.dout.sh, os, lq - q0, oo);
+  };
+  if (it0 < it1) fetch(it0);
+  int bias_head = -1;
+  for (int it = it0; it < it1; ++it) {
+    const int q0 = (tile0 + it % tiles) * IRX_ATTN_BN;
+    const unsigned char* lq_ = smem + ((it - it0) & 1) * 2 * Tile::BYTES;
+    const unsigned char* ld_ = lq_ + Tile::BYTES;
+    float* sm = srow + ((it - it0) & 1) * 3 * IRX_ATTN_BN;
+    float* si = sm + IRX_ATTN_BN;
+    float* se = si + IRX_ATTN_BN;
+    at_landed();
+    if (threadIdx.x < IRX_ATTN_BN) {
+      sm[threadIdx.x] = rm;
+      si[threadIdx.x] = ri;
+      se[threadIdx.x] = rd;
+    }
+    __syncthreads();
+    if (it + 1 < it1) fetch(it + 1);
+    if constexpr (BIAS) {
+      if (bias_head != it / tiles) {                                     // (nobody reads the old one any more: the barrier above)
+        bias_head = it / tiles;
+        at_load_bias<T>(sb, P, kvh * group + bias_head);
+        __syncthreads();
+      }
+    }
+    {
 #pragma unroll
       for (int qb2 = 0; qb2 < 2; ++qb2) {
         const int q1 = q0 + 32 * qb2;
@@ -345,6 +386,18 @@ __global__ __launch_bounds__(256, 1) void k_attn_dkv(AtParams P, int total) {
   }
   if (!mine) return;
   const size_t at = ((size_t)key * P.kv_heads + kvh) * D + 4 * half;
+  if (P.splits > 1) {
+    const size_t one = (size_t)P.tk * P.kv_heads * D;
+    float* ok = P.so + 2 * part * one + at;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        at_st4<AtF32>(ok + 32 * b + 8 * r, dk[b][4 * r], dk[b][4 * r + 1], dk[b][4 * r + 2], dk[b][4 * r + 3]);
+        at_st4<AtF32>(ok + one + 32 * b + 8 * r, dv[b][4 * r], dv[b][4 * r + 1], dv[b][4 * r + 2], dv[b][4 * r + 3]);
+      }
+    return;
+  }
   S* ok = reinterpret_cast<S*>(P.dst) + at;
   S* ov = reinterpret_cast<S*>(P.dst2) + at;
 #pragma unroll
@@ -354,6 +407,19 @@ __global__ __launch_bounds__(256, 1) void k_attn_dkv(AtParams P, int total) {
       at_st4<T>(ok + 32 * b + 8 * r, dk[b][4 * r] * P.scale, dk[b][4 * r + 1] * P.scale, dk[b][4 * r + 2] * P.scale, dk[b][4 * r + 3] * P.scale);
       at_st4<T>(ov + 32 * b + 8 * r, dv[b][4 * r] * (1.f / UP), dv[b][4 * r + 1] * (1.f / UP), dv[b][4 * r + 2] * (1.f / UP), dv[b][4 * r + 3] * (1.f / UP));
     }
+}
+
+// adds the parts of dk and dv in their order and rounds
+template <class T>
+__global__ __launch_bounds__(256) void k_attn_dkv_join(AtParams P, size_t one) {
+  const size_t at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= 2 * one) return;
+  const bool is_v = at >= one;
+  at_f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < P.splits; ++p) s += *reinterpret_cast<const at_f32x4*>(P.so + 2 * p * one + at);
+  const float f = is_v ? (T::ID == IRX_ATTN_F16 ? 1.f / 1024.f : 1.f) : P.scale;
+  typename T::S* to = reinterpret_cast<typename T::S*>(is_v ? P.dst2 : P.dst) + (is_v ? at - one : at);
+  at_st4<T>(to, s[0] * f, s[1] * f, s[2] * f, s[3] * f);
 }
 
 // ---- bias gradient: distances -> buckets, over all tiles -----------------------------------------------------------------------
@@ -398,12 +464,22 @@ __global__ __launch_bounds__(256) void k_attn_dbias(const float* part, int slots
   }
 }
 
+// Parts of the query axis for dk / dv: one, unless there are fewer workgroups (128 keys of one key head each) than compute units can hold.
+static int dkv_splits(long long tq, long long tk, int batch, int heads, int kv_heads) {
+  if (batch <= 0 || tk <= 0 || tq <= 0) return 1;
+  const long long wgs = (tk / IRX_ATTN_BM + (batch < tk ? batch : tk)) * kv_heads;
+  const long long items = heads / kv_heads * ((tq / batch + IRX_ATTN_BN - 1) / IRX_ATTN_BN);
+  long long s = 1024 / (wgs > 0 ? wgs : 1);
+  if (s > items / 4) s = items / 4;
+  return s < 1 ? 1 : s > 8 ? 8 : (int)s;
+}
+
 template <class T, int D, bool BIAS> static int launch_bwd(AtParams P, void* dq, void* dk, void* dv, void* dtable, hipStream_t st) {
-  const size_t tiles = 2 * AtTile<T, D>::BYTES, w = BIAS ? sizeof(float) * (2 * P.far + 1) : 0;
+  const size_t tiles = 4 * AtTile<T, D>::BYTES, w = BIAS ? sizeof(float) * (2 * P.far + 1) : 0;
   if (P.tq > 0) {
     P.slots = at_slots(P.tq, P.batch, IRX_ATTN_BM);
     P.dst = dq;
-    const size_t lds = tiles + 9 * w;
+    const size_t lds = (BIAS && T::ESZ == 4 && D == 128 ? tiles / 2 : tiles) + 9 * w;
     const long long total = (long long)P.slots * P.heads;
     if (int rc = at_want_lds(reinterpret_cast<const void*>(&k_attn_dq<T, D, BIAS>), lds, "irx_attn_packed_bwd")) return rc;
     k_attn_dq<T, D, BIAS><<<(unsigned)((total + 7) / 8 * 8), 256, lds, st>>>(P, (int)total);
@@ -417,11 +493,17 @@ template <class T, int D, bool BIAS> static int launch_bwd(AtParams P, void* dq,
     P.slots = at_slots(P.tk, P.batch, IRX_ATTN_BM);
     P.dst = dk;
     P.dst2 = dv;
-    const size_t lds = tiles + 3 * IRX_ATTN_BN * sizeof(float) + w;
-    const long long total = (long long)P.slots * P.kv_heads;
+    P.splits = dkv_splits(P.tq, P.tk, P.batch, P.heads, P.kv_heads);
+    const size_t lds = tiles + 6 * IRX_ATTN_BN * sizeof(float) + w;
+    const long long total = (long long)P.slots * P.kv_heads * P.splits;
     if (int rc = at_want_lds(reinterpret_cast<const void*>(&k_attn_dkv<T, D, BIAS>), lds, "irx_attn_packed_bwd")) return rc;
     k_attn_dkv<T, D, BIAS><<<(unsigned)((total + 7) / 8 * 8), 256, lds, st>>>(P, (int)total);
     IRX_CHECK_LAUNCH("irx_attn_packed_bwd(dkv)");
+    if (P.splits > 1) {
+      const size_t one = (size_t)P.tk * P.kv_heads * D;
+      k_attn_dkv_join<T><<<(unsigned)((one / 2 + 255) / 256), 256, 0, st>>>(P, one);
+      IRX_CHECK_LAUNCH("irx_attn_packed_bwd(join)");
+    }
   }
   return IRX_OK;
 }
@@ -432,11 +514,16 @@ template <class T> static int launch_bwd_d(const AtParams& P, int dim, void* dq,
   return dim == 32 ? launch_bwd_b<T, 32>(P, dq, dk, dv, dt, st) : dim == 64 ? launch_bwd_b<T, 64>(P, dq, dk, dv, dt, st) : launch_bwd_b<T, 128>(P, dq, dk, dv, dt, st);
 }
 
-extern "C" size_t irx_attn_packed_bwd_workspace_bytes(int tq, int batch, int heads, int far_or_minus1) {
-  if (tq <= 0 || batch < 0 || heads <= 0) return 0;
-  const size_t delta = (size_t)heads * tq;
-  const size_t part = far_or_minus1 < 0 ? 0 : (size_t)at_slots(tq, batch, IRX_ATTN_BM) * heads * (2 * (size_t)far_or_minus1 + 1);
-  return (delta + part) * sizeof(float);
+// D, then (aligned) the parts of dk and dv, then the bias gradient by distance
+static size_t bwd_delta(int tq, int heads) { return ((size_t)heads * tq + 3) / 4 * 4; }
+static size_t bwd_parts(int tq, int tk, int batch, int heads, int kv_heads, int dim) {
+  const int s = dkv_splits(tq, tk, batch, heads, kv_heads);
+  return s > 1 ? (size_t)s * 2 * tk * kv_heads * dim : 0;
+}
+extern "C" size_t irx_attn_packed_bwd_workspace_bytes(int tq, int tk, int batch, int heads, int kv_heads, int dim, int far) {
+  if (tq <= 0 || tk < 0 || batch < 0 || heads <= 0 || kv_heads <= 0 || dim <= 0) return 0;
+  const size_t part = far < 0 ? 0 : (size_t)at_slots(tq, batch, IRX_ATTN_BM) * heads * (2 * (size_t)far + 1);
+  return (bwd_delta(tq, heads) + bwd_parts(tq, tk, batch, heads, kv_heads, dim) + part) * sizeof(float);
 }
 
 extern "C" int irx_attn_packed_bwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
@@ -459,13 +546,15 @@ extern "C" int irx_attn_packed_bwd(const void* q, long long q_row, long long q_h
   IRX_REQUIRE(tk == 0 || (dk && dv), "irx_attn_packed_bwd: null gradient");
   IRX_REQUIRE(!table || dtable, "irx_attn_packed_bwd: null bias gradient");
   IRX_REQUIRE((((uintptr_t)out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) == 0, "irx_attn_packed_bwd: rows must start on 16 bytes");
-  const size_t need = irx_attn_packed_bwd_workspace_bytes(tq, batch, heads, table ? far : -1);
+  const size_t need = irx_attn_packed_bwd_workspace_bytes(tq, tk, batch, heads, kv_heads, dim, table ? far : -1);
   if (need && (!workspace || workspace_bytes < need)) {
     irx_set_error("irx_attn_packed_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     return IRX_ERR_WORKSPACE;
   }
+  IRX_REQUIRE(((uintptr_t)workspace & 15) == 0, "irx_attn_packed_bwd: workspace must start on 16 bytes");
   P.delta = static_cast<float*>(workspace);
-  P.part = P.delta + (size_t)heads * tq;
+  P.so = P.delta + bwd_delta(tq, heads);
+  P.part = P.so + bwd_parts(tq, tk, batch, heads, kv_heads, dim);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == IRX_ATTN_F32) return launch_bwd_d<AtF32>(P, dim, dq, dk, dv, dtable, st);
   if (dtype == IRX_ATTN_BF16) return launch_bwd_d<AtBf16>(P, dim, dq, dk, dv, dtable, st);

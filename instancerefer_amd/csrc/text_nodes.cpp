@@ -38,7 +38,7 @@ namespace {
 typedef size_t (*attn_fwd_ws_fn)(int, int, int, int, int);
 typedef int (*attn_fwd_fn)(const void*, ll, ll, const void*, ll, ll, const void*, ll, ll, const int32_t*, const int32_t*, int, int, int, int, int, int,
                            int, float, int, const void*, int, const int32_t*, int, int, void*, float*, void*, size_t, void*);
-typedef size_t (*attn_bwd_ws_fn)(int, int, int, int);
+typedef size_t (*attn_bwd_ws_fn)(int, int, int, int, int, int, int);
 typedef int (*attn_bwd_fn)(const void*, ll, ll, const void*, ll, ll, const void*, ll, ll, const void*, ll, ll, const void*, const float*,
                            const int32_t*, const int32_t*, int, int, int, int, int, int, int, float, int, const void*, int, const int32_t*, int, int,
                            void*, void*, void*, void*, void*, size_t, void*);
@@ -64,7 +64,7 @@ inline Tensor bytes(size_t n, const Tensor& like) { return at::empty({(int64_t)n
 // rows and heads are read in place from any strides that keep 16-byte alignment
 inline Tensor rows(const Tensor& t) {
   const int64_t e = t.element_size();
-  if (t.stride(2) == 1 && t.stride(0) * e % 16 == 0 && t.stride(1) * e % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) return t;
+  if (t.stride(2) == 1 && t.stride(0) * e % 16 == 0 && t.stride(0) * e < (1 << 24) && t.stride(1) * e % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) return t;
   return t.clone(at::MemoryFormat::Contiguous);
 }
 
@@ -137,7 +137,7 @@ struct AttnNode : public torch::autograd::Function<AttnNode> {
     const bool b = a.table.defined();
     Tensor dt;
     if (b) dt = tq ? at::empty_like(a.table) : at::zeros_like(a.table);
-    const size_t n = g_text.attn_bwd_ws(tq, a.batch(), heads, a.far());
+    const size_t n = g_text.attn_bwd_ws(tq, tk, a.batch(), heads, kv, dim, a.far());
     const Tensor ws = bytes(n ? n : 16, q);
     check(g_text.attn_bwd(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), a.v.data_ptr(), a.v.stride(0), a.v.stride(1),
                           dout.data_ptr(), dout.stride(0), dout.stride(1), out.data_ptr(), stats.data_ptr<float>(), a.cu_q.data_ptr<int32_t>(),

@@ -90,6 +90,7 @@ def test_position_bias_with_keys_of_their_own_length_and_a_free_map(backend):
     table = torch.randn(5, 2, generator=torch.Generator().manual_seed(1))
     buckets = torch.randint(0, 5, (2 * 512 + 1,), generator=torch.Generator().manual_seed(2), dtype=torch.int32)
     compare([90, 7, 1], [33, 700, 0], 2, 2, 32, "f32", False, table=table, buckets=buckets)
+    compare([90, 200, 1], [33, 700, 0], 2, 1, 128, "f32", True, table=table, buckets=buckets)
     compare([90, 7, 1], [33, 700, 5], 2, 2, 128, "bf16", True, table=table[:, :2], buckets=torch.zeros(1, dtype=torch.int32))
 
 
@@ -184,6 +185,16 @@ def test_few_queries_over_many_keys_in_parts(kind, dim):
     assert _lib.load().irx_attn_packed_fwd_workspace_bytes(sum(lens), sum(klens), 5, 4, dim) > 0
     compare(lens, klens, 4, 2, dim, kind)
     compare([2, 1], [2500, 4000], 2, 2, dim, kind, True, seed=2)
+
+
+def test_keys_shared_by_many_query_heads_in_parts():
+    """few key tiles, many queries: the backward gives each workgroup a part of the queries and joins dk, dv"""
+    from instancerefer_amd import _lib
+    one = _lib.load().irx_attn_packed_bwd_workspace_bytes
+    assert one(1400, 1400, 2, 8, 2, 64, -1) > 8 * 1400 * 4      # more than D alone: the parts
+    for kind, dim in (("bf16", 64), ("f16", 128), ("f32", 32)):
+        compare([900, 500], [900, 500], 8, 2, dim, kind, True, seed=dim)
+    compare([1100, 3], [70, 0], 2, 1, 64, "bf16", False, seed=1)
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
