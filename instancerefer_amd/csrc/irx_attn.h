@@ -17,7 +17,7 @@
 #define IRX_ATTN_WAVES 4                     // waves of a workgroup; each owns 32 rows (queries or keys) of the workgroup's tile
 #define IRX_ATTN_BM (32 * IRX_ATTN_WAVES)    // rows of a workgroup's own tile
 #define IRX_ATTN_BN 64                       // rows of the tile that passes through LDS
-#define IRX_ATTN_MAX_FAR 512                 // largest clipped distance of the bucket map (LDS: 8 (2 far + 1) floats in the backward)
+#define IRX_ATTN_MAX_FAR 512                 // largest clipped distance of the bucket map (LDS: 5 (2 far + 1) floats in the backward)
 
 typedef float at_f32x16 __attribute__((ext_vector_type(16)));
 typedef float at_f32x4 __attribute__((ext_vector_type(4)));

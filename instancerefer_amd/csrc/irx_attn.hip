@@ -104,17 +104,22 @@ __global__ __launch_bounds__(256, (T::ESZ == 4 && D == 128) ? 1 : 2) void k_attn
     }
     // key of register i: k0 + 8 (i / 4) + 4 half + i % 4
     if constexpr (BIAS) {
-      const int lo = k0 - (i0 + 31 + off), hi = k0 + IRX_ATTN_BN - 1 - (i0 + off);      // distances key - query in this tile
-      if (hi <= -P.far || lo >= P.far) {
-        const float b = sb[hi <= -P.far ? 0 : 2 * P.far];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) s[i] = __builtin_fmaf(s[i], c1, b);
-      } else {
-        const int d0 = k0 + 4 * half - (i0 + (lane & 31) + off);
+      for (int kb2 = 0; kb2 < 2; ++kb2) {                                // distances key - query of a 32 x 32 block: lo .. hi
+        const int k1 = k0 + 32 * kb2, lo = k1 - (i0 + 31 + off), hi = k1 + 31 - (i0 + off);
+        const int d0 = k1 + 4 * half - (i0 + (lane & 31) + off);
+        if (hi <= -P.far || lo >= P.far) {
+          const float b = sb[hi <= -P.far ? 0 : 2 * P.far];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int d = d0 + 8 * (i >> 2) + (i & 3);
-          s[i] = __builtin_fmaf(s[i], c1, sb[min(max(d, -P.far), P.far) + P.far]);
+          for (int i = 0; i < 16; ++i) s[16 * kb2 + i] = __builtin_fmaf(s[16 * kb2 + i], c1, b);
+        } else if (lo >= -P.far && hi <= P.far) {
+          const float* b = sb + d0 + P.far;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[16 * kb2 + i] = __builtin_fmaf(s[16 * kb2 + i], c1, b[8 * (i >> 2) + (i & 3)]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[16 * kb2 + i] = __builtin_fmaf(s[16 * kb2 + i], c1, sb[min(max(d0 + 8 * (i >> 2) + (i & 3), -P.far), P.far) + P.far]);
         }
       }
     }

@@ -11,13 +11,37 @@
 
 int at_check(const char* who, const AtParams& P, int dim, int dtype, int elem);
 
-// LDS sum without a returned value (ds_add_f32)
-__device__ __forceinline__ void at_lds_add(float* p, float v) { __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
+// Sums of a 32 x 32 result block (keys down: register 4 g + r of lane half h is key 8 g + 4 h + r; queries across the 32 lanes of a half)
+// along its diagonals: lane p gets the sum over key - query = 31 - p (lane 63: nothing). Key by key the running sums move one lane up and
+// the key's row is added (v_mov wave_shr:1), so the row of key n ends 31 - n lanes above its queries; two chains of 16 keys at once.
+// (An LDS sum per value, ds_add_f32, takes 190 clocks here, one wave at a time: 3 us for such a block and four waves.)
+__device__ __forceinline__ float at_up(float x) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x138, 0xf, 0xf, true)); }
+__device__ __forceinline__ float at_diagonals(const float* x) {
+  float a = 0.f, b = 0.f;
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    at_u32x2 lo[4], hi[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {                                        // both halves' rows into lanes 0..31, zeros above
+      lo[r] = __builtin_bit_cast(at_u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x[4 * g + r]), 0u, false, false));
+      hi[r] = __builtin_bit_cast(at_u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x[8 + 4 * g + r]), 0u, false, false));
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        a = at_up(a) + __uint_as_float(lo[r][h]);
+        b = at_up(b) + __uint_as_float(hi[r][h]);
+      }
+  }
+  const int lane = threadIdx.x & 63;                                     // the first chain's rows still lack 16 lanes
+  const float up = __int_as_float(__builtin_amdgcn_ds_bpermute(((lane - 16) & 63) * 4, __float_as_int(a)));
+  return b + (lane < 16 ? 0.f : up);
+}
 
 // ---- dq, D and the bias gradient by distance ----------------------------------------------------------------------------------
-// Bias gradient: sum of dS over all pairs of one distance. Each wave half owns an LDS array by distance and adds its registers one by
-// one: within one instruction the 32 lanes (consecutive queries, one key) hit 32 different distances, so no two lanes meet and the order
-// of additions is fixed; distances at or beyond the clip are summed in registers.
+// Bias gradient: sum of dS over all pairs of one distance. Each wave owns an LDS array by distance and adds a block's 63 diagonals to it
+// at once, one lane each (no atomics, a fixed order); distances at or beyond the clip are summed in registers.
 template <class T, int D, bool BIAS>
 __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P, int total) {
   typedef AtTile<T, D> Tile;
@@ -29,7 +53,7 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
   constexpr int BUFS = (T::ESZ == 4 && D == 128 && BIAS) ? 1 : 2;
   float* sb = reinterpret_cast<float*>(smem + 2 * BUFS * Tile::BYTES);
   const int W = 2 * P.far + 1;
-  float* sd = sb + W;                                                    // [wave][half][W]
+  float* sd = sb + W;                                                    // [wave][W]
 
   const int per = gridDim.x >> 3;
   const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
@@ -89,9 +113,9 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
   }
   if constexpr (BIAS) {
     at_load_bias<T>(sb, P, head);
-    for (int d = threadIdx.x; d < 8 * W; d += 256) sd[d] = 0.f;
+    for (int d = threadIdx.x; d < 4 * W; d += 256) sd[d] = 0.f;
   }
-  float* mysd = sd + (wave * 2 + half) * W;
+  float* mysd = sd + wave * W + P.far;                                   // indexed by distance
   float below = 0.f, above = 0.f;
 
   at_f32x16 acc[BLOCKS];
@@ -132,15 +156,20 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
         y = at_mma(Tile::row_frag(lv_, 32 * kb2, st), df[st], y);
       }
       float p[16];
-      bool near = false;
+      bool near = false, inside = false;
       const int d0 = k1 + 4 * half - (i0 + (lane & 31) + off);
       if constexpr (BIAS) {
         const int lo = k1 - (i0 + 31 + off), hi = k1 + 31 - (i0 + off);
         near = !(hi <= -P.far || lo >= P.far);
+        inside = lo > -P.far && hi < P.far;
         if (!near) {
           const float b = sb[hi <= -P.far ? 0 : 2 * P.far] - m;
 #pragma unroll
           for (int i = 0; i < 16; ++i) p[i] = at_exp2(__builtin_fmaf(x[i], c1, b)) * inv;
+        } else if (inside) {
+          const float* b = sb + d0 + P.far;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) p[i] = at_exp2(__builtin_fmaf(x[i], c1, b[8 * (i >> 2) + (i & 3)]) - m) * inv;
         } else {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -161,12 +190,12 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
       }
       if constexpr (BIAS) {
         if (near) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int d = d0 + 8 * (i >> 2) + (i & 3);
-            if (d > -P.far && d < P.far) at_lds_add(mysd + d + P.far, p[i]);
-            else if (d <= -P.far) below += p[i];
-            else above += p[i];
+          const float z = at_diagonals(p);
+          const int d = k1 - (i0 + off) + 31 - lane;
+          if (lane < 63) {
+            if (d <= -P.far) below += z;
+            else if (d >= P.far) above += z;
+            else mysd[d] += z;
           }
         } else {
           float s = 0.f;
@@ -189,23 +218,24 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
     }
   }
   if constexpr (BIAS) {
+    __syncthreads();                                                     // (no tile at all: the zeros above are another thread's)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+    for (int o = 32; o > 0; o >>= 1) {
       below += __shfl_xor(below, o, 64);
       above += __shfl_xor(above, o, 64);
     }
-    if ((lane & 31) == 0) {                                              // nobody else adds to the clipped distances
+    if (lane == 0) {                                                     // nobody else adds to the clipped distances
       if (P.far == 0) mysd[0] = below + above;
       else {
-        mysd[0] = below;
-        mysd[2 * P.far] = above;
+        mysd[-P.far] = below;
+        mysd[P.far] = above;
       }
     }
     __syncthreads();
     for (int d = threadIdx.x; d < W; d += 256) {
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) s += sd[w * W + d];
+      for (int w = 0; w < 4; ++w) s += sd[w * W + d];
       P.part[((size_t)slot * P.heads + head) * W + d] = s;
     }
   }
@@ -220,7 +250,7 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
 
 // ---- dk, dv -----------------------------------------------------------------------------------------------------------------------
 template <class T, int D, bool BIAS>
-__global__ __launch_bounds__(256, 1) void k_attn_dkv(AtParams P, int total) {
+__global__ __launch_bounds__(256, (T::ESZ == 2 && D <= 64) ? 2 : 1) void k_attn_dkv(AtParams P, int total) {
   typedef AtTile<T, D> Tile;
   typedef typename T::F F;
   typedef typename T::S S;
@@ -338,9 +368,24 @@ __global__ __launch_bounds__(256, 1) void k_attn_dkv(AtParams P, int total) {
         }
         float p[16], ds[16];
         const int lo = j0 - (q1 + 31 + off), hi = j0 + 31 - (q1 + off);  // distances key - query in this block
-        const bool near = BIAS && !(hi <= -P.far || lo >= P.far);
+        const bool near = BIAS && !(hi <= -P.far || lo >= P.far), inside = lo >= -P.far && hi <= P.far;
         float far_bias = 0.f;
         if constexpr (BIAS) far_bias = sb[hi <= -P.far ? 0 : 2 * P.far];
+        float bias[16];
+        if (near) {                                                      // distance of register i: d0 - 8 (i / 4) - i % 4
+          const int d0 = j - (q1 + 4 * half + off);
+          if (inside) {
+            const float* b = sb + d0 + P.far;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) bias[i] = b[-(8 * (i >> 2) + (i & 3))];
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) bias[i] = sb[min(max(d0 - 8 * (i >> 2) - (i & 3), -P.far), P.far) + P.far];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) bias[i] = far_bias;
+        }
         const bool edge = q1 < wave_full || q1 + 32 > lq;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -351,17 +396,7 @@ __global__ __launch_bounds__(256, 1) void k_attn_dkv(AtParams P, int total) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int i = 4 * r + e;
-            float b = -m4[e];
-            if constexpr (BIAS) {
-              if (near) {
-                const int d = j - (q0 + at + e + off);
-                p[i] = at_exp2(__builtin_fmaf(x[i], c1, sb[min(max(d, -P.far), P.far) + P.far]) - m4[e]) * i4[e];
-              } else {
-                p[i] = at_exp2(__builtin_fmaf(x[i], c1, far_bias + b)) * i4[e];
-              }
-            } else {
-              p[i] = at_exp2(__builtin_fmaf(x[i], c1, b)) * i4[e];
-            }
+            p[i] = at_exp2(BIAS ? __builtin_fmaf(x[i], c1, bias[i]) - m4[e] : __builtin_fmaf(x[i], c1, -m4[e])) * i4[e];
             ds[i] = p[i] * (y[i] - e4[e]);
             if (edge) {
               const int qi = q0 + at + e;
@@ -428,18 +463,23 @@ template <class T>
 __global__ __launch_bounds__(256) void k_attn_dbias(const float* part, int slots, int heads, int far, const int32_t* map, int buckets,
                                                     void* dtable, int table_f32) {
   __shared__ int list[2 * IRX_ATTN_MAX_FAR + 1];
+  __shared__ int kind[2 * IRX_ATTN_MAX_FAR + 1];
   __shared__ int count;
   __shared__ double red[4];
   const int bucket = blockIdx.x, head = blockIdx.y, W = 2 * far + 1;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int d = threadIdx.x; d < W; d += 256) {
+    const int b = map[d];
+    kind[d] = b < 0 ? 0 : (b >= buckets ? buckets - 1 : b);
+  }
+  __syncthreads();
   if (wave == 0) {
     int n = 0;
     for (int base = 0; base < W; base += 64) {
       const int d = base + lane;
-      int b = d < W ? map[d] : -1;
-      if (d < W) b = b < 0 ? 0 : (b >= buckets ? buckets - 1 : b);
-      const unsigned long long hit = __ballot(d < W && b == bucket);
-      if (d < W && b == bucket) list[n + __popcll(hit & ((1ull << lane) - 1))] = d;
+      const bool in = d < W && kind[d < W ? d : 0] == bucket;
+      const unsigned long long hit = __ballot(in);
+      if (in) list[n + __popcll(hit & ((1ull << lane) - 1))] = d;
       n += __popcll(hit);
     }
     if (lane == 0) count = n;
@@ -448,8 +488,9 @@ __global__ __launch_bounds__(256) void k_attn_dbias(const float* part, int slots
   const int c = count;
   double s = 0;
   if (c) {
-    const long long n = (long long)slots * c;
-    for (long long i = threadIdx.x; i < n; i += 256) s += (double)part[((size_t)(i / c) * heads + head) * W + list[i % c]];
+    const int n = slots * c;                                             // slots < 2^25 / heads, c <= 1025
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += 256) s += (double)part[((size_t)(i / c) * heads + head) * W + list[i % c]];
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -479,7 +520,7 @@ template <class T, int D, bool BIAS> static int launch_bwd(AtParams P, void* dq,
   if (P.tq > 0) {
     P.slots = at_slots(P.tq, P.batch, IRX_ATTN_BM);
     P.dst = dq;
-    const size_t lds = (BIAS && T::ESZ == 4 && D == 128 ? tiles / 2 : tiles) + 9 * w;
+    const size_t lds = (BIAS && T::ESZ == 4 && D == 128 ? tiles / 2 : tiles) + 5 * w;
     const long long total = (long long)P.slots * P.heads;
     if (int rc = at_want_lds(reinterpret_cast<const void*>(&k_attn_dq<T, D, BIAS>), lds, "irx_attn_packed_bwd")) return rc;
     k_attn_dq<T, D, BIAS><<<(unsigned)((total + 7) / 8 * 8), 256, lds, st>>>(P, (int)total);

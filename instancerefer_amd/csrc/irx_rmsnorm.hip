@@ -221,12 +221,21 @@ __global__ __launch_bounds__(256) void k_rms_bwd(const void* dy, const void* dh,
       }
     }
   }
-  if constexpr (NV > 0) {
+  if constexpr (NV > 0 && G == 64) {                                     // the four waves' sums of a column, in their order
+    __shared__ float s[4][64 * NV * N];
+    const int wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < N; ++e) s[wave][(t + i * 64) * N + e] = dw[i][e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < cols; c += 256) part[(size_t)blockIdx.x * cols + c] = ((s[0][c] + s[1][c]) + s[2][c]) + s[3][c];
+  } else if constexpr (NV > 0) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (t + i * G < nv)
 #pragma unroll
-        for (int e = 0; e < N; ++e) part[(size_t)grp * cols + (size_t)(t + i * G) * N + e] = dw[i][e];
+        for (int e = 0; e < N; ++e) part[(size_t)blockIdx.x * cols + (size_t)(t + i * G) * N + e] = dw[i][e];
   }
 }
 
@@ -241,20 +250,21 @@ __global__ __launch_bounds__(256) void k_rms_dw(const void* dy, const void* h, c
   part[(size_t)blockIdx.y * cols + c] = s;
 }
 
-// dw[c] = sum of the workgroups' sums, 8 interleaved runs per column, joined in their order
+// dw[c] = sum of the workgroups' sums, 32 interleaved runs per column, joined in their order
 template <int ID>
-__global__ __launch_bounds__(256) void k_rms_dw_join(const float* part, int parts, int cols, void* dw, int w_f32) {
-  __shared__ float s[8][32];
+__global__ __launch_bounds__(1024) void k_rms_dw_join(const float* part, int parts, int cols, void* dw, int w_f32) {
+  __shared__ float s[32][33];
   const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5, c = blockIdx.x * 32 + cx;
   float a = 0.f;
   if (c < cols)
-    for (int p = ry; p < parts; p += 8) a += part[(size_t)p * cols + c];
+#pragma unroll 4
+    for (int p = ry; p < parts; p += 32) a += part[(size_t)p * cols + c];
   s[ry][cx] = a;
   __syncthreads();
   if (ry == 0 && c < cols) {
     float t = s[0][cx];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) t += s[i][cx];
+    for (int i = 1; i < 32; ++i) t += s[i][cx];
     if (w_f32) rms_put<0>(dw, c, t);
     else rms_put<ID>(dw, c, t);
   }
@@ -273,15 +283,11 @@ static RmsForm rms_form(int cols, int dtype, bool aligned) {
   if (v <= 1024) return {n, 256, 4};
   return {n, 256, 0};
 }
-// groups of threads that each walk rows and keep their own column sums
+// workgroups of the backward; each walks rows and leaves one sum per column
 static int rms_groups(long long rows, const RmsForm& f) {
-  if (f.nv == 0) return (int)(rows < 256 ? (rows < 1 ? 1 : rows) : 256);
-  const int per = 256 / f.g;
-  long long wgs = (rows + per - 1) / per;
-  const long long most = RMS_MAX_PARTS / per;
-  if (wgs > most) wgs = most;
-  if (wgs < 1) wgs = 1;
-  return (int)wgs * per;
+  const long long most = f.nv == 0 ? 256 : RMS_MAX_PARTS;
+  const long long wgs = f.nv == 0 ? rows : (rows + 256 / f.g - 1) / (256 / f.g);
+  return (int)(wgs < 1 ? 1 : wgs > most ? most : wgs);
 }
 
 extern "C" size_t irx_rms_norm_bwd_workspace_bytes(long long rows, int cols, int dtype) {
@@ -305,7 +311,7 @@ template <int ID, int N> static void rms_launch_fwd(const RmsForm& f, const void
 template <int ID, int N> static void rms_launch_bwd(const RmsForm& f, int groups, const void* dy, const void* dh, const void* h, const void* w, int wf,
                                                     const float* rstd, long long rows, int cols, void* dx, float* part, hipStream_t st) {
   const long long all = (rows + 256 / f.g - 1) / (256 / f.g);
-  const unsigned grid = f.nv ? (unsigned)(groups / (256 / f.g)) : (unsigned)(all < 4096 ? all : 4096);
+  const unsigned grid = f.nv ? (unsigned)groups : (unsigned)(all < 4096 ? all : 4096);
 #define IRX_RMS(G_, NV_) k_rms_bwd<ID, N, G_, NV_><<<grid, 256, 0, st>>>(dy, dh, h, w, wf, rstd, rows, cols, dx, part)
   if constexpr (N == 1) IRX_RMS(256, 0);
   else if (f.g == 64) { if (f.nv == 1) IRX_RMS(64, 1); else IRX_RMS(64, 2); }
@@ -366,9 +372,9 @@ extern "C" int irx_rms_norm_bwd(const void* dy, const void* dh, const void* h, c
     }
   }
   const unsigned grid = (unsigned)((cols + 31) / 32);
-  if (dtype == 0) k_rms_dw_join<0><<<grid, 256, 0, st>>>(part, groups, cols, dweight, 1);
-  else if (dtype == 1) k_rms_dw_join<1><<<grid, 256, 0, st>>>(part, groups, cols, dweight, weight_f32);
-  else k_rms_dw_join<2><<<grid, 256, 0, st>>>(part, groups, cols, dweight, weight_f32);
+  if (dtype == 0) k_rms_dw_join<0><<<grid, 1024, 0, st>>>(part, groups, cols, dweight, 1);
+  else if (dtype == 1) k_rms_dw_join<1><<<grid, 1024, 0, st>>>(part, groups, cols, dweight, weight_f32);
+  else k_rms_dw_join<2><<<grid, 1024, 0, st>>>(part, groups, cols, dweight, weight_f32);
   IRX_CHECK_LAUNCH("irx_rms_norm_bwd(join)");
   return IRX_OK;
 }
