@@ -91,6 +91,7 @@ __global__ __launch_bounds__(256, (T::ESZ == 4 && D == 128) ? 1 : 2) void k_attn
     const unsigned char* lk_ = smem + ((t - t0) & 1) * 2 * Tile::BYTES;
     const unsigned char* lv_ = lk_ + Tile::BYTES;
     if (k0 >= wave_any) continue;
+    __builtin_amdgcn_iglp_opt(1);                                        // LDS reads between the matrix instructions: 4 % at dimension 128
     float s[32];
 #pragma unroll
     for (int kb2 = 0; kb2 < 2; ++kb2) {

@@ -9,6 +9,8 @@
 // from the stored (rounded) output, as the formula's own terms are no more exact than that.
 #include "irx_attn.h"
 
+#include <type_traits>
+
 int at_check(const char* who, const AtParams& P, int dim, int dtype, int elem);
 
 // Sums of a 32 x 32 result block (keys down: register 4 g + r of lane half h is key 8 g + 4 h + r; queries across the 32 lanes of a half)
@@ -148,6 +150,7 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
       const int k1 = k0 + 32 * kb2;
       if (k1 >= wave_any) break;
       at_f32x16 x, y;
+      __builtin_amdgcn_iglp_opt(1);
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = y[i] = 0.f;
 #pragma unroll
@@ -313,8 +316,14 @@ __global__ __launch_bounds__(256, (T::ESZ == 2 && D <= 64) ? 2 : 1) void k_attn_
   Tile::dma_offsets(qo, qs);
   Tile::dma_offsets(oo, os);
   float rm = 0.f, ri = 0.f, rd = 0.f;                                    // row statistics on their way (threads 0..63)
+  // head of the group and tile of the item that is fetched next / worked on
+  int fg = tiles ? it0 / tiles : 0, ft = it0 - fg * tiles, g = fg, tl = ft;
   auto fetch = [&](int it) __attribute__((always_inline)) {
-    const int head = kvh * group + it / tiles, q0 = (tile0 + it % tiles) * IRX_ATTN_BN;
+    const int head = kvh * group + fg, q0 = (tile0 + ft) * IRX_ATTN_BN;
+    if (++ft == tiles) {
+      ft = 0;
+      ++fg;
+    }
     if (threadIdx.x < IRX_ATTN_BN) {
       const int r = q0 + (int)threadIdx.x;
       rm = ri = rd = 0.f;
@@ -332,7 +341,7 @@ __global__ __launch_bounds__(256, (T::ESZ == 2 && D <= 64) ? 2 : 1) void k_attn_
   if (it0 < it1) fetch(it0);
   int bias_head = -1;
   for (int it = it0; it < it1; ++it) {
-    const int q0 = (tile0 + it % tiles) * IRX_ATTN_BN;
+    const int q0 = (tile0 + tl) * IRX_ATTN_BN;
     const unsigned char* lq_ = smem + ((it - it0) & 1) * 2 * Tile::BYTES;
     const unsigned char* ld_ = lq_ + Tile::BYTES;
     float* sm = srow + ((it - it0) & 1) * 3 * IRX_ATTN_BN;
@@ -341,82 +350,97 @@ __global__ __launch_bounds__(256, (T::ESZ == 2 && D <= 64) ? 2 : 1) void k_attn_
     at_landed();
     if (threadIdx.x < IRX_ATTN_BN) {
       sm[threadIdx.x] = rm;
-      si[threadIdx.x] = ri;
-      se[threadIdx.x] = rd;
+      si[threadIdx.x] = ri * UP;
+      se[threadIdx.x] = rd * (1.f / UP);
     }
     __syncthreads();
     if (it + 1 < it1) fetch(it + 1);
     if constexpr (BIAS) {
-      if (bias_head != it / tiles) {                                     // (nobody reads the old one any more: the barrier above)
-        bias_head = it / tiles;
-        at_load_bias<T>(sb, P, kvh * group + bias_head);
+      if (bias_head != g) {                                              // (nobody reads the old one any more: the barrier above)
+        bias_head = g;
+        at_load_bias<T>(sb, P, kvh * group + g);
         __syncthreads();
       }
     }
-    {
+    if (++tl == tiles) {
+      tl = 0;
+      ++g;
+    }
+    auto scores = [&](int qb2, at_f32x16& x, at_f32x16& y) __attribute__((always_inline)) {
 #pragma unroll
-      for (int qb2 = 0; qb2 < 2; ++qb2) {
-        const int q1 = q0 + 32 * qb2;
-        if (q1 + 31 < wave_any || q1 >= lq || row0 >= sp.end) continue;
-        at_f32x16 x, y;
+      for (int i = 0; i < 16; ++i) x[i] = y[i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = y[i] = 0.f;
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-          x = at_mma(Tile::row_frag(lq_, 32 * qb2, s), kf[s], x);
-          y = at_mma(Tile::row_frag(ld_, 32 * qb2, s), vf[s], y);
-        }
-        float p[16], ds[16];
+      for (int st = 0; st < STEPS; ++st) {
+        x = at_mma(Tile::row_frag(lq_, 32 * qb2, st), kf[st], x);
+        y = at_mma(Tile::row_frag(ld_, 32 * qb2, st), vf[st], y);
+      }
+    };
+    auto weights = [&](auto edge, int qb2, const at_f32x16& x, const at_f32x16& y, F (&pf)[2], F (&sf)[2]) __attribute__((always_inline)) {
+      const int q1 = q0 + 32 * qb2;
+      float bias[16];
+      if constexpr (BIAS) {
         const int lo = j0 - (q1 + 31 + off), hi = j0 + 31 - (q1 + off);  // distances key - query in this block
-        const bool near = BIAS && !(hi <= -P.far || lo >= P.far), inside = lo >= -P.far && hi <= P.far;
-        float far_bias = 0.f;
-        if constexpr (BIAS) far_bias = sb[hi <= -P.far ? 0 : 2 * P.far];
-        float bias[16];
-        if (near) {                                                      // distance of register i: d0 - 8 (i / 4) - i % 4
-          const int d0 = j - (q1 + 4 * half + off);
-          if (inside) {
-            const float* b = sb + d0 + P.far;
+        const int d0 = j - (q1 + 4 * half + off);                        // of register i: d0 - 8 (i / 4) - i % 4
+        if (hi <= -P.far || lo >= P.far) {
+          const float b = sb[hi <= -P.far ? 0 : 2 * P.far];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) bias[i] = b[-(8 * (i >> 2) + (i & 3))];
-          } else {
+          for (int i = 0; i < 16; ++i) bias[i] = b;
+        } else if (lo >= -P.far && hi <= P.far) {
+          const float* b = sb + d0 + P.far;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) bias[i] = sb[min(max(d0 - 8 * (i >> 2) - (i & 3), -P.far), P.far) + P.far];
-          }
+          for (int i = 0; i < 16; ++i) bias[i] = b[-(8 * (i >> 2) + (i & 3))];
         } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) bias[i] = far_bias;
+          for (int i = 0; i < 16; ++i) bias[i] = sb[min(max(d0 - 8 * (i >> 2) - (i & 3), -P.far), P.far) + P.far];
         }
-        const bool edge = q1 < wave_full || q1 + 32 > lq;
+      }
+      float p[16], ds[16];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int at = 32 * qb2 + 8 * r + 4 * half;
-          const at_f32x4 m4 = *reinterpret_cast<const at_f32x4*>(sm + at);
-          const at_f32x4 i4 = *reinterpret_cast<const at_f32x4*>(si + at);
-          const at_f32x4 e4 = *reinterpret_cast<const at_f32x4*>(se + at);
+      for (int r = 0; r < 4; ++r) {
+        const int at = 32 * qb2 + 8 * r + 4 * half;
+        const at_f32x4 m4 = *reinterpret_cast<const at_f32x4*>(sm + at);
+        const at_f32x4 i4 = *reinterpret_cast<const at_f32x4*>(si + at);
+        const at_f32x4 e4 = *reinterpret_cast<const at_f32x4*>(se + at);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = 4 * r + e;
-            p[i] = at_exp2(BIAS ? __builtin_fmaf(x[i], c1, bias[i]) - m4[e] : __builtin_fmaf(x[i], c1, -m4[e])) * i4[e];
-            ds[i] = p[i] * (y[i] - e4[e]);
-            if (edge) {
-              const int qi = q0 + at + e;
-              const bool see = qi >= from && qi < lq;
-              p[i] = see ? p[i] : 0.f;
-              ds[i] = see ? ds[i] : 0.f;
-            }
-            p[i] *= UP;
-          }
-        }
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          const F pf = at_pack<T>(p + 8 * ks), sf = at_pack<T>(ds + 8 * ks);
-#pragma unroll
-          for (int b = 0; b < BLOCKS; ++b) {
-            dv[b] = at_mma(Tile::col_frag(ld_, 32 * qb2 + 16 * ks, b), pf, dv[b]);
-            dk[b] = at_mma(Tile::col_frag(lq_, 32 * qb2 + 16 * ks, b), sf, dk[b]);
+        for (int e = 0; e < 4; ++e) {
+          const int i = 4 * r + e;
+          p[i] = at_exp2(BIAS ? __builtin_fmaf(x[i], c1, bias[i]) - m4[e] : __builtin_fmaf(x[i], c1, -m4[e])) * i4[e];
+          ds[i] = p[i] * __builtin_fmaf(y[i], 1.f / UP, -e4[e]);
+          if constexpr (edge) {
+            const int qi = q0 + at + e;
+            const bool see = qi >= from && qi < lq;
+            p[i] = see ? p[i] : 0.f;
+            ds[i] = see ? ds[i] : 0.f;
           }
         }
       }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        pf[ks] = at_pack<T>(p + 8 * ks);
+        sf[ks] = at_pack<T>(ds + 8 * ks);
+      }
+    };
+    auto sums = [&](int qb2, const F (&pf)[2], const F (&sf)[2]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) {
+          dv[b] = at_mma(Tile::col_frag(ld_, 32 * qb2 + 16 * ks, b), pf[ks], dv[b]);
+          dk[b] = at_mma(Tile::col_frag(lq_, 32 * qb2 + 16 * ks, b), sf[ks], dk[b]);
+        }
+    };
+    if (row0 >= sp.end) continue;
+#pragma unroll
+    for (int qb2 = 0; qb2 < 2; ++qb2) {
+      const int q1 = q0 + 32 * qb2;
+      if (q1 + 31 < wave_any || q1 >= lq) continue;
+      at_f32x16 x, y;
+      F pf[2], sf[2];
+      __builtin_amdgcn_iglp_opt(1);                                      // LDS reads between the matrix instructions: 3 % at dimension 128
+      scores(qb2, x, y);
+      if (q1 < wave_full || q1 + 32 > lq) weights(std::true_type{}, qb2, x, y, pf, sf);
+      else weights(std::false_type{}, qb2, x, y, pf, sf);
+      sums(qb2, pf, sf);
     }
   }
   if (!mine) return;
