@@ -190,10 +190,10 @@ __device__ __forceinline__ void at_dma(at_i32x4 rs, unsigned lds, unsigned off) 
 __device__ __forceinline__ void at_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // ---- LDS images -----------------------------------------------------------------------------------------------------------
-// A tile is BN rows of D elements, as they are in memory; the 16-byte pieces of a row are XOR-swizzled by the row so that neither reads
+// A tile is BN rows (a multiple of 32, at least 4 KB) of D elements, as they are in memory; the 16-byte pieces of a row are XOR-swizzled by the row so that neither reads
 // of one piece from 16 rows (ds_read_b128) nor transposing reads of 64 bytes from four rows meet in a bank (64 banks, 256 bytes a turn).
-template <class T, int D> struct AtTile {
-  enum { RB = D * T::ESZ, PIECES = RB / 16, BYTES = IRX_ATTN_BN * RB };
+template <class T, int D, int BN = IRX_ATTN_BN, int WAVES = IRX_ATTN_WAVES> struct AtTile {
+  enum { RB = D * T::ESZ, PIECES = RB / 16, BYTES = BN * RB };
   __device__ static __forceinline__ int swz(int row) {
     if constexpr (T::ESZ == 2) {
       if constexpr (PIECES == 16) return ((row & 3) << 2) | ((row >> 2) & 3);
@@ -208,22 +208,23 @@ template <class T, int D> struct AtTile {
 
   // A tile's way into LDS: direct loads (16 bytes per lane, 1 KB per instruction, no registers in between). The LDS side is linear, so the
   // swizzle is in the addresses: lane l of chunk c fills piece p of row r and asks for piece p ^ swz(r). Rows from `count` on lie behind
-  // the descriptor's end and arrive as zeros. The four waves take every fourth chunk.
-  enum { CHUNKS = BYTES / 4096 };
+  // the descriptor's end and arrive as zeros. The waves take the chunks in turn (WAVES = 1: a wave's own tile).
+  enum { CHUNKS = BYTES / 1024 / WAVES };
+  static_assert(BYTES % (1024 * WAVES) == 0, "whole chunks");
   __device__ static __forceinline__ void dma_offsets(unsigned (&off)[CHUNKS], long long stride_bytes) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = WAVES == 1 ? 0 : threadIdx.x >> 6, lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
-      const int byte = (4 * i + wave) * 1024 + lane * 16, row = byte / RB, piece = (byte % RB) / 16;
+      const int byte = (WAVES * i + wave) * 1024 + lane * 16, row = byte / RB, piece = (byte % RB) / 16;
       off[i] = (unsigned)row * (unsigned)stride_bytes + (unsigned)((piece ^ swz(row)) * 16);
     }
   }
   __device__ static __forceinline__ void dma(unsigned lds, const void* src, long long stride_bytes, int count, const unsigned (&off)[CHUNKS]) {
-    const unsigned n = count < IRX_ATTN_BN ? (unsigned)(count < 0 ? 0 : count) : IRX_ATTN_BN;
+    const unsigned n = count < BN ? (unsigned)(count < 0 ? 0 : count) : BN;
     const at_i32x4 rs = at_rsrc(src, n ? (n - 1) * (unsigned)stride_bytes + RB : 0);
-    const unsigned at = lds + (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 1024;
+    const unsigned at = lds + (WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 1024;
 #pragma unroll
-    for (int i = 0; i < CHUNKS; ++i) at_dma(rs, at + i * 4096, off[i]);
+    for (int i = 0; i < CHUNKS; ++i) at_dma(rs, at + i * WAVES * 1024, off[i]);
   }
   // A operand, rows row0 + l % 32, values 16 step + 8 (l / 32) .. + 7 of the row
   __device__ static __forceinline__ typename T::F row_frag(const unsigned char* lds, int row0, int step) {

@@ -8,9 +8,16 @@
 // weights are rounded to the operand type for the second product (a relative 2^-9 / 2^-12 per weight, below the output's own rounding).
 #include "irx_attn.h"
 
+// keys of a tile and workgroups per compute unit that the registers have to allow. 32 keys in float32: half the work where descriptions
+// end in the first half of a tile (16 of up to 30 words, dimension 64: 9.7 -> 7.5 us), the same speed on long ones; 16 bits: 64 (long
+// causal prompts, dimension 128: 186 us, with 32 and one more workgroup per unit 207).
+template <class T, int D> constexpr int fwd_bn() { return T::ESZ == 4 ? 32 : 64; }
+template <class T, int D> constexpr int fwd_waves() { return T::ESZ == 4 && D == 128 ? 1 : 2; }
+
 template <class T, int D, bool BIAS>
-__global__ __launch_bounds__(256, (T::ESZ == 4 && D == 128) ? 1 : 2) void k_attn_fwd(AtParams P, int total) {
-  typedef AtTile<T, D> Tile;
+__global__ __launch_bounds__(256, (fwd_waves<T, D>())) void k_attn_fwd(AtParams P, int total) {
+  constexpr int BN = fwd_bn<T, D>(), N = BN / 2;                        // keys of a tile, scores per lane
+  typedef AtTile<T, D, BN> Tile;
   typedef typename T::F F;
   typedef typename T::S S;
   constexpr int STEPS = D / 16, BLOCKS = D / 32;
@@ -44,7 +51,7 @@ __global__ __launch_bounds__(256, (T::ESZ == 4 && D == 128) ? 1 : 2) void k_attn
   const int wave_full = P.causal ? min(lk, i0 + 1 + off) : lk;           // ... to every row of the wave
   const int wave_any = row0 >= sp.end ? 0 : (P.causal ? min(lk, min(i0 + 32, sp.end - first) + off) : lk);
   const int block_any = P.causal ? min(lk, min(sp.begin + IRX_ATTN_BM, sp.end) - first + off) : lk;
-  int t0 = 0, t1 = (max(block_any, 0) + IRX_ATTN_BN - 1) / IRX_ATTN_BN;
+  int t0 = 0, t1 = (max(block_any, 0) + BN - 1) / BN;
   if (P.splits > 1) {
     const int n = t1;
     t0 = (int)((long long)n * part / P.splits);
@@ -78,13 +85,13 @@ __global__ __launch_bounds__(256, (T::ESZ == 4 && D == 128) ? 1 : 2) void k_attn
   Tile::dma_offsets(vo, vs);
   auto fetch = [&](int t) __attribute__((always_inline)) {
     const unsigned to = lds0 + ((t - t0) & 1) * 2 * Tile::BYTES;
-    const int k0 = t * IRX_ATTN_BN;
+    const int k0 = t * BN;
     Tile::dma(to, kp + k0 * P.k.st, ks, lk - k0, ko);
     Tile::dma(to + Tile::BYTES, vp + k0 * P.v.st, vs, lk - k0, vo);
   };
   if (t0 < t1) fetch(t0);
   for (int t = t0; t < t1; ++t) {
-    const int k0 = t * IRX_ATTN_BN;
+    const int k0 = t * BN;
     at_landed();
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
@@ -92,9 +99,9 @@ __global__ __launch_bounds__(256, (T::ESZ == 4 && D == 128) ? 1 : 2) void k_attn
     const unsigned char* lv_ = lk_ + Tile::BYTES;
     if (k0 >= wave_any) continue;
     __builtin_amdgcn_iglp_opt(1);                                        // LDS reads between the matrix instructions: 4 % at dimension 128
-    float s[32];
+    float s[N];
 #pragma unroll
-    for (int kb2 = 0; kb2 < 2; ++kb2) {
+    for (int kb2 = 0; kb2 < BN / 32; ++kb2) {
       at_f32x16 x;
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = 0.f;
@@ -106,7 +113,7 @@ __global__ __launch_bounds__(256, (T::ESZ == 4 && D == 128) ? 1 : 2) void k_attn
     // key of register i: k0 + 8 (i / 4) + 4 half + i % 4
     if constexpr (BIAS) {
 #pragma unroll
-      for (int kb2 = 0; kb2 < 2; ++kb2) {                                // distances key - query of a 32 x 32 block: lo .. hi
+      for (int kb2 = 0; kb2 < BN / 32; ++kb2) {                                // distances key - query of a 32 x 32 block: lo .. hi
         const int k1 = k0 + 32 * kb2, lo = k1 - (i0 + 31 + off), hi = k1 + 31 - (i0 + off);
         const int d0 = k1 + 4 * half - (i0 + (lane & 31) + off);
         if (hi <= -P.far || lo >= P.far) {
@@ -124,14 +131,14 @@ __global__ __launch_bounds__(256, (T::ESZ == 4 && D == 128) ? 1 : 2) void k_attn
         }
       }
     }
-    if (k0 + IRX_ATTN_BN > wave_full) {
+    if (k0 + BN > wave_full) {
       const int left = lim - k0 - 4 * half;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) s[i] = 8 * (i >> 2) + (i & 3) < left ? s[i] : -INFINITY;
+      for (int i = 0; i < N; ++i) s[i] = 8 * (i >> 2) + (i & 3) < left ? s[i] : -INFINITY;
     }
     float mx = s[0];
 #pragma unroll
-    for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i]);
+    for (int i = 1; i < N; ++i) mx = fmaxf(mx, s[i]);
     mx = at_pair_max(mx);
     if constexpr (!BIAS) mx *= c1;                                       // c1 > 0
     // the running maximum moves only when a row outgrows it by 2^8: weights stay below 256, and most tiles rescale nothing
@@ -148,13 +155,13 @@ __global__ __launch_bounds__(256, (T::ESZ == 4 && D == 128) ? 1 : 2) void k_attn
     const float ms = m == -INFINITY ? 0.f : m;
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < N; ++i) {
       s[i] = at_exp2(BIAS ? s[i] - ms : __builtin_fmaf(s[i], c1, -ms));
       sum += s[i];
     }
     l += sum;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
+    for (int ks = 0; ks < BN / 16; ++ks) {
       const F p = at_pack<T>(s + 8 * ks);
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) acc[b] = at_mma(Tile::col_frag(lv_, 16 * ks, b), p, acc[b]);
@@ -190,57 +197,214 @@ __global__ __launch_bounds__(256, (T::ESZ == 4 && D == 128) ? 1 : 2) void k_attn
   }
 }
 
-// joins the parts of a row: o = sum_p w_p o_p / sum_p w_p, w_p = l_p 2^(m_p - max m); parts in their order, so always the same result
+// Few queries over many keys (single tokens, a handful of instances): the queries of ALL heads that share a key head are one tile of 32
+// rows (row = token * group + head of the group), so keys and values are read once per key head, and every wave walks keys of its own:
+// tiles of 32 keys through a buffer that only this wave uses, two in turn, no barrier. Bound by reading keys and values; each wave leaves
+// a partial result.
+template <class T, int D> constexpr int few_waves() { return T::ESZ == 4 && D == 128 ? 2 : 4; }   // LDS: 64 KB per wave there, 32 KB at most else
+
+template <class T, int D>
+__global__ __launch_bounds__((64 * few_waves<T, D>())) void k_attn_few(AtParams P, int total, int tokens) {
+  constexpr int WV = few_waves<T, D>(), STEPS = D / 16, BLOCKS = D / 32;
+  typedef AtTile<T, D, 32, 1> Tile;
+  typedef typename T::F F;
+  typedef typename T::S S;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int per = gridDim.x >> 3;
+  const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (id >= total) return;
+  const int shares = P.splits / WV;                                      // workgroups of one (tile, key head)
+  const int share = id % shares, rest = id / shares, kvh = rest % P.kv_heads, slot = rest / P.kv_heads;
+  int first;
+  const AtSpan sp = at_span(P.cu_q, P.batch, P.tq, tokens, slot, &first);
+  if (sp.begin >= sp.end) return;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int kb = 0, ke = 0;
+  if (sp.seq >= 0) {
+    kb = __builtin_amdgcn_readfirstlane(at_edge(P.cu_k, P.batch, P.tk, sp.seq + 1));
+    ke = __builtin_amdgcn_readfirstlane(at_edge(P.cu_k, P.batch, P.tk, sp.seq + 2));
+  }
+  const int lk = ke > kb ? ke - kb : 0, off = lk - (sp.end - first);
+  const int group = P.heads / P.kv_heads;
+  const int row = lane & 31, token = row / group, head = kvh * group + row % group;
+  const int q = sp.begin + token;
+  const bool mine = token < tokens && q < sp.end;
+  const int lim = !mine ? 0 : P.causal ? max(0, min(lk, q - first + 1 + off)) : lk;
+  const int full = P.causal ? min(lk, sp.begin - first + 1 + off) : lk;  // keys that every row sees
+  const int any = P.causal ? max(0, min(lk, min(sp.begin + tokens, sp.end) - first + off)) : lk;
+  const int part = share * WV + wave, n = (any + 31) / 32;
+  const int t0 = (int)((long long)n * part / P.splits), t1 = (int)((long long)n * (part + 1) / P.splits);
+  const S* kp = reinterpret_cast<const S*>(P.k.p) + kb * P.k.st + kvh * P.k.sh;
+  const S* vp = reinterpret_cast<const S*>(P.v.p) + kb * P.v.st + kvh * P.v.sh;
+  const float c1 = P.scale * IRX_LOG2E;
+  const long long ks = P.k.st * T::ESZ, vs = P.v.st * T::ESZ;
+  unsigned ko[Tile::CHUNKS], vo[Tile::CHUNKS];
+  Tile::dma_offsets(ko, ks);
+  Tile::dma_offsets(vo, vs);
+  unsigned char* buf = smem + wave * 4 * Tile::BYTES;
+  const unsigned lds0 = at_lds_addr(buf);
+
+  F qf[STEPS];
+  {
+    const S* qp = reinterpret_cast<const S*>(P.q.p) + q * P.q.st + head * P.q.sh + 8 * half;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) qf[s] = mine ? at_ldg<T>(qp + 16 * s) : at_zero<T>();
+  }
+  at_f32x16 acc[BLOCKS];
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  auto fetch = [&](int t) __attribute__((always_inline)) {
+    const unsigned to = lds0 + ((t - t0) & 1) * 2 * Tile::BYTES;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                   // the buffer's last readers are back
+    Tile::dma(to, kp + (long long)t * 32 * P.k.st, ks, lk - t * 32, ko);
+    Tile::dma(to + Tile::BYTES, vp + (long long)t * 32 * P.v.st, vs, lk - t * 32, vo);
+  };
+  at_landed();                                                           // (the queries: from here on only tiles are on their way)
+  if (t0 < t1) fetch(t0);
+  for (int t = t0; t < t1; ++t) {
+    if (t + 1 < t1) {
+      fetch(t + 1);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * Tile::CHUNKS) : "memory");      // everything but that tile
+    } else {
+      at_landed();
+    }
+    const unsigned char* lk_ = buf + ((t - t0) & 1) * 2 * Tile::BYTES;
+    const unsigned char* lv_ = lk_ + Tile::BYTES;
+    at_f32x16 x;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = 0.f;
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) x = at_mma(Tile::row_frag(lk_, 0, st), qf[st], x);
+    float s[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = x[i];
+    if (t * 32 + 32 > full) {
+      const int left = lim - t * 32 - 4 * half;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = 8 * (i >> 2) + (i & 3) < left ? s[i] : -INFINITY;
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    mx = at_pair_max(mx) * c1;
+    if (__any(mx > m + 8.f || m == -INFINITY)) {
+      const float mn = fmaxf(m, mx);
+      const float a = mn == -INFINITY ? 1.f : at_exp2(m - mn);
+      m = mn;
+      l *= a;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[b][i] *= a;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = at_exp2(__builtin_fmaf(s[i], c1, -ms));
+      l += s[i];
+    }
+#pragma unroll
+    for (int k2 = 0; k2 < 2; ++k2) {
+      const F p = at_pack<T>(s + 8 * k2);
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) acc[b] = at_mma(Tile::col_frag(lv_, 16 * k2, b), p, acc[b]);
+    }
+  }
+  l = at_pair_sum(l);
+  if (!mine) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const size_t r = ((size_t)part * P.heads + head) * P.tq + q;
+  float* o = P.so + r * D + 4 * half;
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      at_st4<AtF32>(o + 32 * b + 8 * g, acc[b][4 * g] * inv, acc[b][4 * g + 1] * inv, acc[b][4 * g + 2] * inv, acc[b][4 * g + 3] * inv);
+  if (half == 0) {
+    P.sst[2 * r] = m;
+    P.sst[2 * r + 1] = l;
+  }
+}
+
+// Joins the parts of a row: o = sum_p w_p o_p / sum_p w_p, w_p = l_p 2^(m_p - max m). One workgroup per row (head, query): groups of
+// D / 4 threads take every G-th part, their sums are joined in the groups' order: always the same result.
 template <class T, int D>
 __global__ __launch_bounds__(256) void k_attn_join(AtParams P) {
-  constexpr int PER = D / 4;
-  const size_t n = (size_t)P.heads * P.tq * PER, at = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= n) return;
-  const size_t row = at / PER;                                           // head * tq + q
-  const int d = (int)(at % PER) * 4;
-  const size_t rows = (size_t)P.heads * P.tq;
+  constexpr int PER = D / 4, G = 256 / PER;
+  __shared__ at_f32x4 so[G][PER];
+  __shared__ float sl[G];
+  const size_t row = blockIdx.x, rows = (size_t)P.heads * P.tq;          // head * tq + q
+  const int c = threadIdx.x % PER, g = threadIdx.x / PER, d = 4 * c;
   float M = -INFINITY;
+#pragma unroll 4
   for (int p = 0; p < P.splits; ++p) M = fmaxf(M, P.sst[2 * (p * rows + row)]);
   const float Ms = M == -INFINITY ? 0.f : M;
   float L = 0.f;
   at_f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int p = 0; p < P.splits; ++p) {
+#pragma unroll 4
+  for (int p = g; p < P.splits; p += G) {
     const float l = P.sst[2 * (p * rows + row) + 1];
-    if (l == 0.f) continue;
-    const float w = l * at_exp2(P.sst[2 * (p * rows + row)] - Ms);
     const at_f32x4 x = *reinterpret_cast<const at_f32x4*>(P.so + (p * rows + row) * D + d);
+    const float w = l == 0.f ? 0.f : l * at_exp2(P.sst[2 * (p * rows + row)] - Ms);
     L += w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(w, x[i], o[i]);
   }
+  so[g][c] = o;
+  if (c == 0) sl[g] = L;
+  __syncthreads();
+  if (g) return;
+  L = sl[0];
+#pragma unroll
+  for (int i = 1; i < G; ++i) {
+    L += sl[i];
+    o += so[i][c];
+  }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   const size_t head = row / P.tq, q = row % P.tq;
   at_st4<T>(reinterpret_cast<typename T::S*>(P.dst) + (q * P.heads + head) * D + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-  if (P.wstats && d == 0) {
+  if (P.wstats && c == 0) {
     P.wstats[2 * row] = Ms;
     P.wstats[2 * row + 1] = inv;
   }
 }
 
+template <class T, int D> static int launch_join(const AtParams& P, hipStream_t st) {
+  k_attn_join<T, D><<<(unsigned)((size_t)P.heads * P.tq), 256, 0, st>>>(P);
+  IRX_CHECK_LAUNCH("irx_attn_packed_fwd(join)");
+  return IRX_OK;
+}
+
+template <class T, int D> static int launch_few(AtParams P, int tokens, hipStream_t st) {
+  const size_t lds = (size_t)few_waves<T, D>() * 4 * AtTile<T, D, 32, 1>::BYTES;
+  P.slots = at_slots(P.tq, P.batch, tokens);
+  const long long total = (long long)P.slots * P.kv_heads * (P.splits / few_waves<T, D>());
+  if (int rc = at_want_lds(reinterpret_cast<const void*>(&k_attn_few<T, D>), lds, "irx_attn_packed_fwd")) return rc;
+  k_attn_few<T, D><<<(unsigned)((total + 7) / 8 * 8), 64 * few_waves<T, D>(), lds, st>>>(P, (int)total, tokens);
+  IRX_CHECK_LAUNCH("irx_attn_packed_fwd(few)");
+  return launch_join<T, D>(P, st);
+}
+
 template <class T, int D, bool BIAS> static int launch_fwd(const AtParams& P, hipStream_t st) {
-  const size_t lds = 4 * AtTile<T, D>::BYTES + (BIAS ? sizeof(float) * (2 * P.far + 1) : 0);
+  const size_t lds = 4 * AtTile<T, D, fwd_bn<T, D>()>::BYTES + (BIAS ? sizeof(float) * (2 * P.far + 1) : 0);
   const long long total = (long long)P.slots * P.heads * P.splits;
   const unsigned grid = (unsigned)((total + 7) / 8 * 8);
   if (int rc = at_want_lds(reinterpret_cast<const void*>(&k_attn_fwd<T, D, BIAS>), lds, "irx_attn_packed_fwd")) return rc;
   k_attn_fwd<T, D, BIAS><<<grid, 256, lds, st>>>(P, (int)total);
   IRX_CHECK_LAUNCH("irx_attn_packed_fwd");
-  if (P.splits > 1) {
-    const size_t n = (size_t)P.heads * P.tq * (D / 4);
-    k_attn_join<T, D><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(P);
-    IRX_CHECK_LAUNCH("irx_attn_packed_fwd(join)");
-  }
-  return IRX_OK;
+  return P.splits > 1 ? launch_join<T, D>(P, st) : IRX_OK;
 }
-template <class T, int D> static int launch_fwd_b(const AtParams& P, hipStream_t st) {
+template <class T, int D> static int launch_fwd_b(const AtParams& P, int tokens, hipStream_t st) {
+  if (tokens) return launch_few<T, D>(P, tokens, st);
   return P.table ? launch_fwd<T, D, true>(P, st) : launch_fwd<T, D, false>(P, st);
 }
-template <class T> static int launch_fwd_d(const AtParams& P, int dim, hipStream_t st) {
-  return dim == 32 ? launch_fwd_b<T, 32>(P, st) : dim == 64 ? launch_fwd_b<T, 64>(P, st) : launch_fwd_b<T, 128>(P, st);
+template <class T> static int launch_fwd_d(const AtParams& P, int dim, int tokens, hipStream_t st) {
+  return dim == 32 ? launch_fwd_b<T, 32>(P, tokens, st) : dim == 64 ? launch_fwd_b<T, 64>(P, tokens, st) : launch_fwd_b<T, 128>(P, tokens, st);
 }
 
 int at_check(const char* who, const AtParams& P, int dim, int dtype, int elem) {
@@ -270,19 +434,32 @@ int at_check(const char* who, const AtParams& P, int dim, int dtype, int elem) {
   return IRX_OK;
 }
 
-// Parts of the key axis: one, unless the whole launch is far below one workgroup per compute unit and there are many keys per sequence.
-static int fwd_splits(long long tq, long long tk, int batch, int heads) {
-  if (batch <= 0 || tk <= 0) return 1;
-  const long long wgs = (tq / IRX_ATTN_BM + (batch < tq ? batch : tq)) * heads, keys = tk / batch;
-  if (wgs >= 512 || keys < 1024) return 1;
-  long long s = 1024 / (wgs > 0 ? wgs : 1);
+// How the forward is launched, by sizes alone. Few: the average sequence's queries, times the heads that share a key head, fit one tile
+// of 32 rows, and there are many keys (16 single tokens over 500 to 8100 keys, 16 / 4 heads of 128: 24 us, without it 83). Else parts of
+// the key axis only where the whole launch is far below one workgroup per compute unit. tokens: queries of a few-row tile, 0: no.
+struct FwdPlan { int tokens, splits; };
+static FwdPlan fwd_plan(long long tq, long long tk, int batch, int heads, int kv_heads, int dim, int elem, bool bias) {
+  if (batch <= 0 || tk <= 0 || tq <= 0) return {0, 1};
+  const long long keys = tk / batch, busy = batch < tq ? batch : tq;
+  const int group = heads / kv_heads;
+  if (!bias && group <= 32 && tq <= (long long)batch * (32 / group) && keys >= 512) {
+    const int tokens = 32 / group, waves = elem == 4 && dim == 128 ? 2 : 4;
+    long long s = (512 + busy * kv_heads - 1) / (busy * kv_heads);
+    if (s > keys / 256) s = keys / 256;
+    if (s < 1) s = 1;
+    if (s > 16) s = 16;
+    return {tokens, (int)s * waves};
+  }
+  const long long wgs = (tq / IRX_ATTN_BM + busy) * heads;
+  if (wgs >= 512 || keys < 1024) return {0, 1};
+  long long s = 1024 / wgs;
   if (s > keys / 256) s = keys / 256;
-  return s < 1 ? 1 : s > 32 ? 32 : (int)s;
+  return {0, s < 1 ? 1 : s > 32 ? 32 : (int)s};
 }
 
-extern "C" size_t irx_attn_packed_fwd_workspace_bytes(int tq, int tk, int batch, int heads, int dim) {
-  if (tq <= 0 || tk < 0 || batch < 0 || heads <= 0 || dim <= 0) return 0;
-  const int s = fwd_splits(tq, tk, batch, heads);
+extern "C" size_t irx_attn_packed_fwd_workspace_bytes(int tq, int tk, int batch, int heads, int kv_heads, int dim, int dtype, int bias) {
+  if (tq <= 0 || tk < 0 || batch < 0 || heads <= 0 || kv_heads <= 0 || dim <= 0) return 0;
+  const int s = fwd_plan(tq, tk, batch, heads, kv_heads, dim, dtype == IRX_ATTN_F32 ? 4 : 2, bias != 0).splits;
   return s <= 1 ? 0 : (size_t)s * heads * tq * (dim + 2) * sizeof(float);
 }
 
@@ -303,9 +480,10 @@ extern "C" int irx_attn_packed_fwd(const void* q, long long q_row, long long q_h
   if (tq == 0) return IRX_OK;
   IRX_REQUIRE(out && ((uintptr_t)out & 15) == 0, "irx_attn_packed_fwd: out must be given and start on 16 bytes");
   P.slots = at_slots(tq, batch, IRX_ATTN_BM);
-  P.splits = fwd_splits(tq, tk, batch, heads);
+  const FwdPlan plan = fwd_plan(tq, tk, batch, heads, kv_heads, dim, dtype == IRX_ATTN_F32 ? 4 : 2, table != nullptr);
+  P.splits = plan.splits;
   if (P.splits > 1) {
-    const size_t need = irx_attn_packed_fwd_workspace_bytes(tq, tk, batch, heads, dim);
+    const size_t need = irx_attn_packed_fwd_workspace_bytes(tq, tk, batch, heads, kv_heads, dim, dtype, table != nullptr);
     if (!workspace || workspace_bytes < need) {
       irx_set_error("irx_attn_packed_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
       return IRX_ERR_WORKSPACE;
@@ -315,9 +493,9 @@ extern "C" int irx_attn_packed_fwd(const void* q, long long q_row, long long q_h
     P.sst = P.so + (size_t)P.splits * heads * tq * dim;
   }
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == IRX_ATTN_F32) return launch_fwd_d<AtF32>(P, dim, st);
-  if (dtype == IRX_ATTN_BF16) return launch_fwd_d<AtBf16>(P, dim, st);
-  return launch_fwd_d<AtF16>(P, dim, st);
+  if (dtype == IRX_ATTN_F32) return launch_fwd_d<AtF32>(P, dim, plan.tokens, st);
+  if (dtype == IRX_ATTN_BF16) return launch_fwd_d<AtBf16>(P, dim, plan.tokens, st);
+  return launch_fwd_d<AtF16>(P, dim, plan.tokens, st);
 }
 
 extern "C" int irx_stream_capturing(void* stream) {

@@ -35,7 +35,7 @@ static int64_t foreign_leaf(const std::vector<OptTensor>& leaves) {
 
 namespace {
 
-typedef size_t (*attn_fwd_ws_fn)(int, int, int, int, int);
+typedef size_t (*attn_fwd_ws_fn)(int, int, int, int, int, int, int, int);
 typedef int (*attn_fwd_fn)(const void*, ll, ll, const void*, ll, ll, const void*, ll, ll, const int32_t*, const int32_t*, int, int, int, int, int, int,
                            int, float, int, const void*, int, const int32_t*, int, int, void*, float*, void*, size_t, void*);
 typedef size_t (*attn_bwd_ws_fn)(int, int, int, int, int, int, int);
@@ -101,7 +101,7 @@ Tensor attn_forward(const Attn& a, Tensor* stats, void* stream) {
   const int tq = (int)q.size(0), heads = (int)q.size(1), dim = (int)q.size(2), tk = (int)k.size(0), kv = (int)k.size(1);
   Tensor out = at::empty({tq, heads, dim}, q.options());
   if (stats) *stats = at::empty({heads, tq, 2}, q.options().dtype(at::kFloat));
-  const size_t n = g_text.attn_fwd_ws(tq, tk, a.batch(), heads, dim);
+  const size_t n = g_text.attn_fwd_ws(tq, tk, a.batch(), heads, kv, dim, type_of(q), a.table.defined());
   const Tensor ws = n ? bytes(n, q) : Tensor();
   const bool b = a.table.defined();
   check(g_text.attn_fwd(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), a.v.data_ptr(), a.v.stride(0), a.v.stride(1),

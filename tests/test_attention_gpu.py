@@ -182,9 +182,24 @@ def test_strided_views_and_other_head_dimensions(kind, backend):
 def test_few_queries_over_many_keys_in_parts(kind, dim):
     from instancerefer_amd import _lib
     lens, klens = [1, 3, 1, 0, 2], [3000, 1, 1500, 700, 0]
-    assert _lib.load().irx_attn_packed_fwd_workspace_bytes(sum(lens), sum(klens), 5, 4, dim) > 0
+    assert _lib.load().irx_attn_packed_fwd_workspace_bytes(sum(lens), sum(klens), 5, 4, 2, dim, 0, 0) > 0
     compare(lens, klens, 4, 2, dim, kind)
     compare([2, 1], [2500, 4000], 2, 2, dim, kind, True, seed=2)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv", [(3, 1), (32, 1), (40, 1), (5, 5), (12, 4)])
+def test_few_queries_of_every_grouping(kind, heads, kv):
+    """rows of a few-query tile are (token, head of the group): groups that do not divide 32, that fill it, that exceed it; one sequence
+    with more queries than a tile holds among short ones; causal with more queries than keys"""
+    compare([1, 14, 2, 1, 1, 0], [900, 700, 40, 2500, 1, 33], heads, kv, 32, kind, False, seed=heads)
+    compare([1, 14, 5, 1, 1, 0, 1, 1, 1, 1], [900, 700, 3, 2500, 1, 33, 900, 0, 800, 1000], heads, kv, 64, kind, True, seed=heads)
+
+
+def test_few_queries_with_a_bias_in_parts():
+    from instancerefer_amd.attention import relative_buckets
+    table = torch.randn(8, 2, generator=torch.Generator().manual_seed(3))
+    compare([1, 2], [3000, 2600], 2, 1, 64, "bf16", False, table=table, buckets=relative_buckets(8, 30))
 
 
 def test_keys_shared_by_many_query_heads_in_parts():

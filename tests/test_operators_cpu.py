@@ -117,8 +117,8 @@ def test_c_entries_refuse(lib):
         assert call(**kw) == -1, kw
         assert b"irx_attn_packed_fwd" in lib.irx_last_error()
     assert call(tq=0) == 0
-    assert lib.irx_attn_packed_fwd_workspace_bytes(16, 16, 1, 4, 64) == 0
-    need = lib.irx_attn_packed_fwd_workspace_bytes(1, 8000, 1, 4, 64)
+    assert lib.irx_attn_packed_fwd_workspace_bytes(16, 16, 1, 4, 4, 64, 0, 0) == 0
+    need = lib.irx_attn_packed_fwd_workspace_bytes(1, 8000, 1, 4, 2, 64, 0, 0)
     assert need > 0 and need % ((64 + 2) * 4 * 4) == 0
     assert f(one, 256, 64, one, 128, 64, one, 128, 64, one, one, 1, 1, 8000, 4, 2, 64, 0, 0.1, 0, None, 1, None, 0, 0, one, None, None, 0, None) == -3
     assert lib.irx_attn_packed_bwd_workspace_bytes(100, 100, 2, 4, 4, 64, -1) == 100 * 4 * 4
