@@ -654,7 +654,7 @@ int irx_attn_packed_fwd(const void* q, long long q_row, long long q_head, const 
                         int tk, int heads, int kv_heads, int dim, int dtype, float scale, int causal, const void* table,
                         int table_f32, const int32_t* map, int buckets, int far, void* out, float* stats, void* workspace,
                         size_t workspace_bytes, void* stream);
-size_t irx_attn_packed_bwd_workspace_bytes(int tq, int tk, int batch, int heads, int kv_heads, int dim, int far);
+size_t irx_attn_packed_bwd_workspace_bytes(int tq, int tk, int batch, int heads, int kv_heads, int dim, int dtype, int far);
 int irx_attn_packed_bwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
                         const void* v, long long v_row, long long v_head, const void* dout, long long do_row, long long do_head,
                         const void* out, const float* stats, const int32_t* cu_q, const int32_t* cu_k, int batch, int tq, int tk,

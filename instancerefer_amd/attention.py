@@ -131,7 +131,7 @@ class AttentionPackedFn(torch.autograd.Function):
         if table is not None:
             dt = torch.empty_like(table) if tq else torch.zeros_like(table)
         tb, tb_f32, mp, nb, far = _table_args(table, buckets)
-        n = int(_lib.load().irx_attn_packed_bwd_workspace_bytes(tq, tk, batch, heads, kv_heads, dim, far))
+        n = int(_lib.load().irx_attn_packed_bwd_workspace_bytes(tq, tk, batch, heads, kv_heads, dim, _TYPES[q.dtype], far))
         ws = torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
         _lib.call("irx_attn_packed_bwd", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
                   v.stride(0), v.stride(1), dout.data_ptr(), dout.stride(0), dout.stride(1), out.data_ptr(), stats.data_ptr(),

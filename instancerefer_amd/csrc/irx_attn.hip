@@ -435,7 +435,7 @@ int at_check(const char* who, const AtParams& P, int dim, int dtype, int elem) {
 }
 
 // How the forward is launched, by sizes alone. Few: the average sequence's queries, times the heads that share a key head, fit one tile
-// of 32 rows, and there are many keys (16 single tokens over 500 to 8100 keys, 16 / 4 heads of 128: 24 us, without it 83). Else parts of
+// of 32 rows, and there are many keys (16 single tokens over 500 to 8100 keys, 16 / 4 heads of 128: 35 us with the join, without it 83; about 256 workgroups: 512 41, 1024 51). Else parts of
 // the key axis only where the whole launch is far below one workgroup per compute unit. tokens: queries of a few-row tile, 0: no.
 struct FwdPlan { int tokens, splits; };
 static FwdPlan fwd_plan(long long tq, long long tk, int batch, int heads, int kv_heads, int dim, int elem, bool bias) {
@@ -444,7 +444,7 @@ static FwdPlan fwd_plan(long long tq, long long tk, int batch, int heads, int kv
   const int group = heads / kv_heads;
   if (!bias && group <= 32 && tq <= (long long)batch * (32 / group) && keys >= 512) {
     const int tokens = 32 / group, waves = elem == 4 && dim == 128 ? 2 : 4;
-    long long s = (512 + busy * kv_heads - 1) / (busy * kv_heads);
+    long long s = (256 + busy * kv_heads - 1) / (busy * kv_heads);
     if (s > keys / 256) s = keys / 256;
     if (s < 1) s = 1;
     if (s > 16) s = 16;

@@ -38,7 +38,7 @@ namespace {
 typedef size_t (*attn_fwd_ws_fn)(int, int, int, int, int, int, int, int);
 typedef int (*attn_fwd_fn)(const void*, ll, ll, const void*, ll, ll, const void*, ll, ll, const int32_t*, const int32_t*, int, int, int, int, int, int,
                            int, float, int, const void*, int, const int32_t*, int, int, void*, float*, void*, size_t, void*);
-typedef size_t (*attn_bwd_ws_fn)(int, int, int, int, int, int, int);
+typedef size_t (*attn_bwd_ws_fn)(int, int, int, int, int, int, int, int);
 typedef int (*attn_bwd_fn)(const void*, ll, ll, const void*, ll, ll, const void*, ll, ll, const void*, ll, ll, const void*, const float*,
                            const int32_t*, const int32_t*, int, int, int, int, int, int, int, float, int, const void*, int, const int32_t*, int, int,
                            void*, void*, void*, void*, void*, size_t, void*);
@@ -137,7 +137,7 @@ struct AttnNode : public torch::autograd::Function<AttnNode> {
     const bool b = a.table.defined();
     Tensor dt;
     if (b) dt = tq ? at::empty_like(a.table) : at::zeros_like(a.table);
-    const size_t n = g_text.attn_bwd_ws(tq, tk, a.batch(), heads, kv, dim, a.far());
+    const size_t n = g_text.attn_bwd_ws(tq, tk, a.batch(), heads, kv, dim, type_of(q), a.far());
     const Tensor ws = bytes(n ? n : 16, q);
     check(g_text.attn_bwd(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), a.v.data_ptr(), a.v.stride(0), a.v.stride(1),
                           dout.data_ptr(), dout.stride(0), dout.stride(1), out.data_ptr(), stats.data_ptr<float>(), a.cu_q.data_ptr<int32_t>(),

@@ -206,7 +206,7 @@ def test_keys_shared_by_many_query_heads_in_parts():
     """few key tiles, many queries: the backward gives each workgroup a part of the queries and joins dk, dv"""
     from instancerefer_amd import _lib
     one = _lib.load().irx_attn_packed_bwd_workspace_bytes
-    assert one(1400, 1400, 2, 8, 2, 64, -1) > 8 * 1400 * 4      # more than D alone: the parts
+    assert one(1400, 1400, 2, 8, 2, 64, 1, -1) > 8 * 1400 * 4      # more than D alone: the parts
     for kind, dim in (("bf16", 64), ("f16", 128), ("f32", 32)):
         compare([900, 500], [900, 500], 8, 2, dim, kind, True, seed=dim)
     compare([1100, 3], [70, 0], 2, 1, 64, "bf16", False, seed=1)

@@ -121,8 +121,8 @@ def test_c_entries_refuse(lib):
     need = lib.irx_attn_packed_fwd_workspace_bytes(1, 8000, 1, 4, 2, 64, 0, 0)
     assert need > 0 and need % ((64 + 2) * 4 * 4) == 0
     assert f(one, 256, 64, one, 128, 64, one, 128, 64, one, one, 1, 1, 8000, 4, 2, 64, 0, 0.1, 0, None, 1, None, 0, 0, one, None, None, 0, None) == -3
-    assert lib.irx_attn_packed_bwd_workspace_bytes(100, 100, 2, 4, 4, 64, -1) == 100 * 4 * 4
-    assert lib.irx_attn_packed_bwd_workspace_bytes(100, 100, 2, 4, 4, 64, 8) > 100 * 4 * 4
+    assert lib.irx_attn_packed_bwd_workspace_bytes(100, 100, 2, 4, 4, 64, 0, -1) == 100 * 4 * 4
+    assert lib.irx_attn_packed_bwd_workspace_bytes(100, 100, 2, 4, 4, 64, 0, 8) > 100 * 4 * 4
     assert lib.irx_attn_packed_bwd(one, 256, 64, one, 128, 64, one, 128, 64, one, 256, 64, one, one, one, one, 1, 8, 8, 4, 2, 64, 0, 0.1, 0, None, 1, None,
                                    0, 0, one, one, one, None, None, 0, None) == -3
     assert lib.irx_rms_norm_fwd(one, None, one, 1, 4, 0, 0, 1e-6, one, None, None, None) == -1
