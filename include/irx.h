@@ -613,18 +613,19 @@ int irx_adam_step(float* params, const float* grads, float* exp_avg, float* exp_
  *
  * irx_clip_grads: scales n_tensors tensors in place and writes the norm BEFORE clipping to norm[0] (device float). Host arrays of device
  *   pointers, types (0 float32, 1 bf16, 2 fp16) and element counts; a tensor is one contiguous range, two tensors must not share memory.
- * irx_grad_norm_parts + irx_adam_step_clip: the same for ONE flat float32 buffer inside the optimizer: the first leaves partial sums of
- *   grads[0, n) in workspace, the second is irx_adam_step with the gradients multiplied by grad_scale * factor as they are read (no
- *   clipped gradients are written); norm_parts = that workspace, norm_values = that n, and the norm counts grad_scale. norm (may be
- *   NULL): device float. With a factor of 1 it computes what irx_adam_step does. */
+ * irx_grad_gather_norm + irx_adam_step_clip: the same for the optimizer's flat float32 buffer. The first copies n_tensors tensors to their
+ *   places (src == dst: only read) and leaves partial sums in workspace, irx_grad_gather_parts() doubles and one more; the second is
+ *   irx_adam_step with the gradients multiplied by grad_scale * factor as they are read (no clipped gradients are written). The norm
+ *   counts grad_scale; norm (may be NULL): device float. With a factor of 1 it computes what irx_adam_step does. */
 size_t irx_clip_grads_workspace_bytes(const unsigned long long* counts_host, int n_tensors);
 int irx_clip_grads(void* const* grads_host, const int* types_host, const unsigned long long* counts_host, int n_tensors, int inf_norm,
                    float max_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream);
-size_t irx_grad_norm_workspace_bytes(size_t n);
-int irx_grad_norm_parts(const float* grads, size_t n, int inf_norm, void* workspace, size_t workspace_bytes, void* stream);
+size_t irx_grad_gather_parts(const unsigned long long* counts_host, int n_tensors);
+int irx_grad_gather_norm(const float* const* src_host, float* const* dst_host, const unsigned long long* counts_host, int n_tensors,
+                         int inf_norm, void* workspace, size_t workspace_bytes, void* stream);
 int irx_adam_step_clip(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, size_t n, float lr, float beta1,
                        float beta2, float eps, float weight_decay, int step, float grad_scale, const void* norm_parts,
-                       size_t norm_values, int inf_norm, float max_norm, float* norm, void* stream);
+                       size_t n_parts, int inf_norm, float max_norm, float* norm, void* stream);
 
 /* Root-mean-square norm with the residual's addition. Types: 0 float32, 1 bf16, 2 fp16; weight float32 (weight_f32) or the same type.
  *   fwd: h = x + residual rounded to the type (residual NULL: h is x and is not written), rstd = 1 / sqrt(mean(h^2) + eps) over cols,

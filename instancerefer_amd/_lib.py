@@ -116,8 +116,8 @@ _SIGNATURES = {
     "irx_iou_labels": (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P]),
     "irx_clip_grads_workspace_bytes": (_Z, [_P, _I]),
     "irx_clip_grads": (_I, [_P, _P, _P, _I, _I, _F, _P, _P, _Z, _P]),
-    "irx_grad_norm_workspace_bytes": (_Z, [_Z]),
-    "irx_grad_norm_parts": (_I, [_P, _Z, _I, _P, _Z, _P]),
+    "irx_grad_gather_parts": (_Z, [_P, _I]),
+    "irx_grad_gather_norm": (_I, [_P, _P, _P, _I, _I, _P, _Z, _P]),
     "irx_adam_step_clip": (_I, [_P, _P, _P, _P, _Z, _F, _F, _F, _F, _F, _I, _F, _P, _Z, _I, _F, _P, _P]),
     "irx_rms_norm_fwd": (_I, [_P, _P, _P, _I, _L, _I, _I, _F, _P, _P, _P, _P]),
     "irx_rms_norm_bwd_workspace_bytes": (_Z, [_L, _I, _I]),

@@ -364,37 +364,118 @@ __global__ __launch_bounds__(256) void k_adam_clip(float* __restrict__ p, const 
   }
 }
 
-extern "C" size_t irx_grad_norm_workspace_bytes(size_t n) {
-  const unsigned long long c = clip_chunk(n);
-  return (size_t)((n + c - 1) / c + 1) * sizeof(double);
+// ---- gathering the gradients into the flat buffer, with their norm ----
+// The copy that the optimizer's gather is, and the sum of squares on the way: one read and one write, no second pass for the norm. A
+// tensor that already lies in its place (src == dst) is only read.
+#define IRX_GATHER_TENSORS 128               // 3.6 KB of kernel arguments
+struct GatherTable {
+  const float* src[IRX_GATHER_TENSORS];
+  float* dst[IRX_GATHER_TENSORS];
+  unsigned long long n[IRX_GATHER_TENSORS];
+  int first[IRX_GATHER_TENSORS + 1];
+  int count;
+};
+
+__global__ __launch_bounds__(256) void k_gather_norm(GatherTable T, unsigned long long chunk, int inf, double* parts) {
+  __shared__ double red[4];
+  int t = 0, top = T.count - 1;
+  while (t < top) {
+    const int mid = (t + top + 1) >> 1;
+    if (T.first[mid] <= (int)blockIdx.x) t = mid;
+    else top = mid - 1;
+  }
+  const size_t lo = (size_t)(blockIdx.x - T.first[t]) * chunk;
+  const size_t hi = lo + chunk < T.n[t] ? lo + chunk : T.n[t];
+  const float* src = T.src[t];
+  float* dst = T.dst[t];
+  const bool copy = src != dst;
+  double a[4] = {0, 0, 0, 0};
+  size_t i = lo;
+  if (((((uintptr_t)src) | ((uintptr_t)dst)) & 15) == 0) {
+    const size_t end = lo + (hi - lo) / 4 * 4;
+    for (i = lo + (size_t)threadIdx.x * 4; i < end; i += 1024) {
+      const float4 v = *reinterpret_cast<const float4*>(src + i);
+      if (copy) *reinterpret_cast<float4*>(dst + i) = v;
+      clip_take(a[0], v.x, inf);
+      clip_take(a[1], v.y, inf);
+      clip_take(a[2], v.z, inf);
+      clip_take(a[3], v.w, inf);
+    }
+    i = end;
+  }
+  for (i += threadIdx.x; i < hi; i += 256) {
+    const float v = src[i];
+    if (copy) dst[i] = v;
+    clip_take(a[0], v, inf);
+  }
+  const double s = clip_block(clip_join(clip_join(a[0], a[1], inf), clip_join(a[2], a[3], inf), inf), inf, red);
+  if (threadIdx.x == 0) parts[blockIdx.x] = s;
 }
 
-extern "C" int irx_grad_norm_parts(const float* grads, size_t n, int inf_norm, void* workspace, size_t workspace_bytes, void* stream) {
-  IRX_REQUIRE(n == 0 || grads, "irx_grad_norm_parts: null pointer");
-  IRX_REQUIRE(((uintptr_t)grads & 3) == 0 && n < ((size_t)1 << 48), "irx_grad_norm_parts: bad gradients");
-  const size_t need = irx_grad_norm_workspace_bytes(n);
-  if (!workspace || workspace_bytes < need) {
-    irx_set_error("irx_grad_norm_parts: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+static unsigned long long gather_chunk(const unsigned long long* counts, int n, unsigned long long* parts) {
+  unsigned long long total = 0, k = 0;
+  for (int i = 0; i < n; ++i) total += counts[i];
+  const unsigned long long c = clip_chunk(total);
+  for (int i = 0; i < n; ++i) k += (counts[i] + c - 1) / c;
+  *parts = k;
+  return c;
+}
+
+extern "C" size_t irx_grad_gather_parts(const unsigned long long* counts_host, int n_tensors) {
+  if (!counts_host || n_tensors <= 0) return 0;
+  unsigned long long k;
+  gather_chunk(counts_host, n_tensors, &k);
+  return (size_t)k;
+}
+
+extern "C" int irx_grad_gather_norm(const float* const* src_host, float* const* dst_host, const unsigned long long* counts_host, int n_tensors,
+                                    int inf_norm, void* workspace, size_t workspace_bytes, void* stream) {
+  IRX_REQUIRE(n_tensors >= 0 && (n_tensors == 0 || (src_host && dst_host && counts_host)), "irx_grad_gather_norm: null table");
+  for (int i = 0; i < n_tensors; ++i) {
+    IRX_REQUIRE(counts_host[i] < (1ull << 40), "irx_grad_gather_norm: tensor %d has too many values", i);
+    IRX_REQUIRE(counts_host[i] == 0 || (src_host[i] && dst_host[i]), "irx_grad_gather_norm: tensor %d is null", i);
+    IRX_REQUIRE((((uintptr_t)src_host[i] | (uintptr_t)dst_host[i]) & 3) == 0, "irx_grad_gather_norm: tensor %d is not aligned to 4 bytes", i);
+  }
+  if (n_tensors == 0) return IRX_OK;
+  unsigned long long k;
+  const unsigned long long c = gather_chunk(counts_host, n_tensors, &k);
+  if (!workspace || workspace_bytes < (k + 1) * sizeof(double)) {
+    irx_set_error("irx_grad_gather_norm: workspace of %zu bytes, %llu needed", workspace_bytes, (k + 1) * 8);
     return IRX_ERR_WORKSPACE;
   }
-  IRX_REQUIRE(((uintptr_t)workspace & 7) == 0, "irx_grad_norm_parts: workspace must start on 8 bytes");
-  if (n == 0) return IRX_OK;
-  const unsigned long long c = clip_chunk(n);
-  ClipTable T;
-  T.count = 1;
-  T.p[0] = const_cast<float*>(grads);
-  T.n[0] = n;
-  T.first[0] = 0;
-  T.first[1] = (int)((n + c - 1) / c);
-  T.type[0] = ((uintptr_t)grads & 15) == 0 ? 4 : 0;
-  k_clip_norm<<<T.first[1], 256, 0, (hipStream_t)stream>>>(T, c, inf_norm, static_cast<double*>(workspace));
-  IRX_CHECK_LAUNCH("irx_grad_norm_parts");
+  IRX_REQUIRE(((uintptr_t)workspace & 7) == 0, "irx_grad_gather_norm: workspace must start on 8 bytes");
+  double* parts = static_cast<double*>(workspace);
+  hipStream_t st = (hipStream_t)stream;
+  GatherTable T;
+  int done = 0;
+  for (int i = 0; i < n_tensors;) {
+    T.count = 0;
+    int chunks = 0;
+    for (; i < n_tensors && T.count < IRX_GATHER_TENSORS; ++i) {
+      if (!counts_host[i]) continue;
+      const int t = T.count++;
+      T.src[t] = src_host[i];
+      T.dst[t] = dst_host[i];
+      T.n[t] = counts_host[i];
+      T.first[t] = chunks;
+      chunks += (int)((counts_host[i] + c - 1) / c);
+    }
+    if (!T.count) break;
+    T.first[T.count] = chunks;
+    k_gather_norm<<<chunks, 256, 0, st>>>(T, c, inf_norm, parts + done);
+    IRX_CHECK_LAUNCH("irx_grad_gather_norm");
+    done += chunks;
+  }
+  if (done > 2 * IRX_CLIP_PARTS) {
+    k_clip_fold<<<1, 256, 0, st>>>(parts, done, inf_norm, parts + done);
+    IRX_CHECK_LAUNCH("irx_grad_gather_norm(fold)");
+  }
   return IRX_OK;
 }
 
 extern "C" int irx_adam_step_clip(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, size_t n, float lr, float beta1,
                                   float beta2, float eps, float weight_decay, int step, float grad_scale, const void* norm_parts,
-                                  size_t norm_values, int inf_norm, float max_norm, float* norm, void* stream) {
+                                  size_t n_parts, int inf_norm, float max_norm, float* norm, void* stream) {
   IRX_REQUIRE(step >= 1, "irx_adam_step_clip: step must be >= 1");
   IRX_REQUIRE(max_norm >= 0.f, "irx_adam_step_clip: the largest norm must be >= 0");
   if (n == 0) return IRX_OK;
@@ -403,13 +484,14 @@ extern "C" int irx_adam_step_clip(float* params, const float* grads, float* exp_
               "irx_adam_step_clip: buffers must be 16-byte aligned");
   const double bc1 = 1.0 - pow((double)beta1, (double)step);
   const double bc2 = 1.0 - pow((double)beta2, (double)step);
-  const unsigned long long c = clip_chunk(norm_values);
+  const double* parts = static_cast<const double*>(norm_parts);
+  const bool folded = n_parts > 2 * IRX_CLIP_PARTS;                      // their sum lies behind them
   long long blocks = (long long)((n / 4 + 255) / 256);
   if (blocks > 2048) blocks = 2048;
   if (blocks < 1) blocks = 1;
   k_adam_clip<<<(int)blocks, 256, 0, (hipStream_t)stream>>>(params, grads, exp_avg, exp_avg_sq, n, lr, beta1, beta2, eps, weight_decay, (float)bc1,
-                                                             (float)sqrt(bc2), grad_scale, static_cast<const double*>(norm_parts),
-                                                             (int)((norm_values + c - 1) / c), inf_norm, max_norm, norm);
+                                                             (float)sqrt(bc2), grad_scale, folded ? parts + n_parts : parts, folded ? 1 : (int)n_parts,
+                                                             inf_norm, max_norm, norm);
   IRX_CHECK_LAUNCH("irx_adam_step_clip");
   return IRX_OK;
 }

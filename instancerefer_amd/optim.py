@@ -67,6 +67,12 @@ def _clip_args(who, max_norm, norm_type):
     return max_norm, int(norm_type == math.inf)
 
 
+def _norm_table(dst, counts):
+    n = len(counts)
+    c = (ctypes.c_ulonglong * n)(*counts)
+    return (ctypes.c_void_p * n)(*dst), c, n, int(_lib.load().irx_grad_gather_parts(c, n))
+
+
 @torch.no_grad()
 def clip_grads_(grads, max_norm, norm_type=2.0):
     """Clip the GLOBAL norm of a list of gradients to max_norm, in place (csrc/irx_optim.hip): every value is multiplied by
@@ -179,6 +185,7 @@ class FlatAdam:
         self._direct = set()            # parameter indices whose slot already holds this step's gradient
         self._direct_groups = set()     # producer keys that delivered since the last zero_grad()
         self._gather_cache = {}
+        self._slot_at, self._table_cache = None, {}      # addresses of the slots and the tables of irx_grad_gather_norm (clipping)
         self._pending = []              # sink deliveries not yet waited for: (event | (lane, stream), parameter indices)
         self._todo_last = list(range(len(self.params)))
         self._works = []                # async collectives in flight
@@ -311,8 +318,10 @@ class FlatAdam:
         # ordering of the product path can be exercised on a single GPU
         return dist.is_initialized() and (self.world_size > 1 or getattr(self, "_force_collectives", False))
 
-    def gather_grads(self):
-        """All .grad tensors -> their slots in flat_g with one multi-tensor copy (the padding between slots stays zero;
+    def gather_grads(self, sum_norm=None):
+        """sum_norm None. (0 / 1: the copy is irx_grad_gather_norm, which also sums the squares / takes the largest magnitude of ALL
+        gradients, those already in their slots included; -> the partial sums. One rank only: nothing is reduced in between.)
+        All .grad tensors -> their slots in flat_g with one multi-tensor copy (the padding between slots stays zero;
         a missing grad leaves a zero slot and marks the parameter inactive for this step); slots already filled through
         the sink protocol are left alone. In overlap mode with world_size > 1, each delivered group that is one
         contiguous range of flat_g is all-reduced right here, on the producer's stream, before the copy of the remaining
@@ -375,16 +384,49 @@ class FlatAdam:
             else:
                 slots.append(self._slots[i])
                 grads.append(g)
-        if slots:
+        sums = None
+        self._inactive = frozenset(inactive)
+        if sum_norm is not None:
+            sums = self._gather_and_sum([i for i in todo if i not in self._inactive] if inactive else todo, grads, sum_norm)
+        elif slots:
             torch._foreach_copy_(slots, grads)
         if zero:
             torch._foreach_zero_(zero)
-        self._inactive = frozenset(inactive)
+        if sum_norm is not None:
+            return sums
         for i in self._direct:           # a producer delivered AND autograd accumulated (second backward): add it
             g = self.params[i].grad
             if g is not None:
                 self._slots[i].add_(g)
                 self.params[i].grad = None
+
+    def _gather_and_sum(self, todo, grads, inf_norm):
+        """grads[k] -> the slot of parameter todo[k] with one launch (per 128), and the sums of those and of the slots already filled."""
+        direct = sorted(self._direct)
+        for i in direct:                 # a producer delivered AND autograd accumulated (second backward): add it
+            g = self.params[i].grad
+            if g is not None:
+                self._slots[i].add_(g)
+                self.params[i].grad = None
+        if self._slot_at is None:
+            self._slot_at = [t.data_ptr() for t in self._slots]
+        at = self._slot_at
+        key = (tuple(direct), tuple(todo))
+        ent = self._table_cache.get(key)
+        if ent is None:                  # places and sizes stay the same from step to step
+            if len(self._table_cache) > 16:
+                self._table_cache.clear()
+            idx = direct + list(todo)
+            ent = self._table_cache[key] = _norm_table([at[i] for i in idx], [self._slots[i].numel() for i in idx])
+        f32, dev = torch.float32, self.device
+        src = [at[i] for i in direct]
+        for i, g in zip(todo, grads):
+            if g.dtype is f32 and g.is_contiguous() and g.device == dev:
+                src.append(g.data_ptr())
+            else:
+                self._slots[i].copy_(g)
+                src.append(at[i])
+        return self._norm_parts(src, ent, inf_norm)
 
     def all_reduce(self):
         """Sum flat_g over the ranks (the division by world_size happens in the Adam kernel): the static segments in order,
@@ -445,22 +487,34 @@ class FlatAdam:
                       float(self.betas[0]), float(self.betas[1]), float(self.eps), float(self.weight_decay), step,
                       1.0 / self.world_size, _lib.stream_ptr())
 
-    def _step_clipped(self, max_norm, inf_norm):
-        lib = _lib.load()
-        nb = int(lib.irx_grad_norm_workspace_bytes(self.n))
-        ws = torch.empty(nb, dtype=torch.uint8, device=self.device)
+    def _norm_parts(self, src, table, inf_norm):
+        """Copies from the addresses src to the table's (equal: only read) and -> (workspace with the partial sums of their norm, how many)."""
+        dst, counts, n, parts = table
+        ws = torch.empty(parts + 1, dtype=torch.float64, device=self.device)
+        _lib.call("irx_grad_gather_norm", (ctypes.c_void_p * n)(*src), dst, counts, n, inf_norm, ws.data_ptr(), 8 * (parts + 1),
+                  _lib.stream_ptr())
+        return ws, parts
+
+    def _step_clipped(self, max_norm, inf_norm, sums=None):
+        if sums is None:
+            at = _lib.ptr(self.flat_g)
+            sums = self._norm_parts([at], _norm_table([at], [self.n]), inf_norm)
+        ws, parts = sums
         norm = torch.empty((), dtype=torch.float32, device=self.device)
-        _lib.call("irx_grad_norm_parts", _lib.ptr(self.flat_g), self.n, inf_norm, ws.data_ptr(), nb, _lib.stream_ptr())
         runs = self._runs()
         for lo, hi, step in runs:
             _lib.call("irx_adam_step_clip", _lib.ptr(self.flat_p[lo:hi]), _lib.ptr(self.flat_g[lo:hi]),
                       _lib.ptr(self.exp_avg[lo:hi]), _lib.ptr(self.exp_avg_sq[lo:hi]), hi - lo, float(self.lr),
                       float(self.betas[0]), float(self.betas[1]), float(self.eps), float(self.weight_decay), step,
-                      1.0 / self.world_size, ws.data_ptr(), self.n, inf_norm, max_norm, norm.data_ptr(), _lib.stream_ptr())
+                      1.0 / self.world_size, ws.data_ptr(), parts, inf_norm, max_norm, norm.data_ptr(), _lib.stream_ptr())
         return norm if runs else norm.zero_()           # (no parameter had a gradient)
 
     def backward_step(self, max_norm=None, norm_type=2.0):
-        """After loss.backward(): gather -> all-reduce -> (clip ->) Adam. Returns what step() returns."""
+        """After loss.backward(): gather -> all-reduce -> (clip ->) Adam. Returns what step() returns. With max_norm on one rank the norm
+        is summed while the gradients are gathered."""
+        if max_norm is not None and self.device.type == "cuda" and not self._multi_rank():
+            max_norm, inf_norm = _clip_args("FlatAdam.backward_step", max_norm, norm_type)
+            return self._step_clipped(max_norm, inf_norm, self.gather_grads(inf_norm))
         self.gather_grads()
         self.all_reduce()
         return self.step(max_norm, norm_type)

@@ -188,6 +188,32 @@ def test_parameters_without_gradients_and_none_at_all():
     assert all(torch.equal(p, b) for p, b in zip(ps, before))
 
 
+def test_gather_of_gradients_of_every_layout_and_of_many_tensors():
+    """transposed, expanded, off 16 bytes, more tensors than one table and more sums than one fold: as if gathered first"""
+    from instancerefer_amd.optim import FlatAdam
+    for shapes in ([(40, 30), (7, 9), (50,), (3, 5)], [(1 + i % 7,) for i in range(2300)]):
+        one, two = params_of(shapes, 5), params_of(shapes, 5)
+        a, b = FlatAdam(one, lr=1e-2), FlatAdam(two, lr=1e-2)
+        g = torch.Generator().manual_seed(6)
+        for i, (p, q) in enumerate(zip(one, two)):
+            x = torch.randn(p.shape, generator=g).to(DEV)
+            if i == 0 and p.dim() == 2:
+                x = x.t().contiguous().t()
+            elif i == 1 and p.dim() == 2:
+                x = x[:1].expand(p.shape)
+            elif i == 2:
+                buf = torch.empty(x.numel() + 1, device=DEV)[1:]
+                buf.copy_(x)
+                x = buf.view(x.shape)
+            p.grad, q.grad = x, x.clone()
+        a.gather_grads()
+        want = a.step(max_norm=0.3)                                     # gathered, then summed over the flat buffer
+        got = b.backward_step(max_norm=0.3)                             # summed on the way
+        assert torch.equal(a.flat_g, b.flat_g)
+        assert abs(float(got) - float(want)) <= 4 * 2.0 ** -24 * float(want)
+        assert float((a.flat_p - b.flat_p).abs().max()) <= 1e-2 * 64 * 2.0 ** -24 + 2.0 ** -23 * float(a.flat_p.abs().max())
+
+
 def test_norm_counts_the_mean_over_ranks():
     from instancerefer_amd.optim import FlatAdam
     ps = params_of([(50,)], 4)

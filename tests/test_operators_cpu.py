@@ -139,4 +139,8 @@ def test_c_entries_refuse(lib):
     types[1] = 3
     assert lib.irx_clip_grads(apart, types, counts, 2, 0, 1.0, one, one, 1 << 20, None) == -1
     assert lib.irx_adam_step_clip(one, one, one, one, 4, 1e-3, 0.9, 0.99, 1e-8, 0.0, 0, 1.0, one, 4, 0, 1.0, one, None) == -1
-    assert lib.irx_grad_norm_parts(one, 100, 0, None, 0, None) == -3
+    assert lib.irx_grad_gather_parts(counts, 2) == 2 and lib.irx_grad_gather_parts(None, 0) == 0
+    assert lib.irx_grad_gather_norm(apart, apart, counts, 2, 0, None, 0, None) == -3
+    odd = (ctypes.c_void_p * 2)(4098, 4136)
+    assert lib.irx_grad_gather_norm(odd, apart, counts, 2, 0, one, 1 << 10, None) == -1
+    assert lib.irx_grad_gather_norm(None, None, None, 0, 0, None, 0, None) == 0
