@@ -647,19 +647,20 @@ int irx_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* 
  *   bias (table != NULL) = table[map[far + clamp(j - (i + Lk - Lq), -far, far)]][h]; table [buckets][heads] float32 (table_f32) or the
  *   tensors' type, map int32 [2 far + 1] (device, far <= 512).
  * out, dq [tq][heads][dim], dk, dv [tk][kv_heads][dim] contiguous; stats float32 [heads][tq][2] is what the backward needs of the
- * forward (NULL: not written); dtable like table. Offsets are read on the device only: no length has to be known on the host.
+ * forward (NULL: not written); rest, like out and in 16 bits only: what out's rounding left over, which makes the gradients more exact
+ * (NULL in the forward: not kept, in the backward: none); dtable like table. Offsets are read on the device only: no length has to be known on the host.
  * Deterministic. irx_attn_packed_bwd_workspace_bytes: far = -1 without a bias table. */
 size_t irx_attn_packed_fwd_workspace_bytes(int tq, int tk, int batch, int heads, int kv_heads, int dim, int dtype, int bias);
 int irx_attn_packed_fwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
                         const void* v, long long v_row, long long v_head, const int32_t* cu_q, const int32_t* cu_k, int batch, int tq,
                         int tk, int heads, int kv_heads, int dim, int dtype, float scale, int causal, const void* table,
-                        int table_f32, const int32_t* map, int buckets, int far, void* out, float* stats, void* workspace,
+                        int table_f32, const int32_t* map, int buckets, int far, void* out, void* rest, float* stats, void* workspace,
                         size_t workspace_bytes, void* stream);
 size_t irx_attn_packed_bwd_workspace_bytes(int tq, int tk, int batch, int heads, int kv_heads, int dim, int dtype, int far);
 int irx_attn_packed_bwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
                         const void* v, long long v_row, long long v_head, const void* dout, long long do_row, long long do_head,
-                        const void* out, const float* stats, const int32_t* cu_q, const int32_t* cu_k, int batch, int tq, int tk,
-                        int heads, int kv_heads, int dim, int dtype, float scale, int causal, const void* table, int table_f32,
+                        const void* out, const void* rest, const float* stats, const int32_t* cu_q, const int32_t* cu_k, int batch,
+                        int tq, int tk, int heads, int kv_heads, int dim, int dtype, float scale, int causal, const void* table, int table_f32,
                         const int32_t* map, int buckets, int far, void* dq, void* dk, void* dv, void* dtable, void* workspace,
                         size_t workspace_bytes, void* stream);
 

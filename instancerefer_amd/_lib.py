@@ -124,10 +124,10 @@ _SIGNATURES = {
     "irx_rms_norm_bwd": (_I, [_P, _P, _P, _P, _I, _P, _L, _I, _I, _P, _P, _P, _Z, _P]),
     "irx_attn_packed_fwd_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I, _I, _I]),
     "irx_attn_packed_fwd": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _I, _P, _I, _I, _P, _P, _P,
-                                 _Z, _P]),
+                                 _P, _Z, _P]),
     "irx_attn_packed_bwd_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I, _I, _I]),
-    "irx_attn_packed_bwd": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _I, _P,
-                                 _I, _I, _P, _P, _P, _P, _P, _Z, _P]),
+    "irx_attn_packed_bwd": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _I,
+                                 _P, _I, _I, _P, _P, _P, _P, _P, _Z, _P]),
     "irx_eval_select": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P]),
 }
 

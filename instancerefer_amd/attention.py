@@ -15,7 +15,8 @@ over every key j of the sequence or, with `causal`, j <= i + Lk - Lq (the last q
 zeros and takes no gradient; so do rows outside every sequence (behind cu[-1]).
 
 Types: float32 (products in float32), bfloat16, float16; scores, softmax and sums are float32, the softmax's weights and the score gradients
-are rounded to the tensors' type where they enter the second products. Float16 gradients of scores below 6e-8 vanish: scale the loss.
+are rounded to the tensors' type where they enter the second products. In 16 bits a forward that will be differentiated keeps a second tensor
+of the output's size, what its rounding left over, for the gradients' sake. Float16 gradients of scores below 6e-8 vanish: scale the loss.
 Keys of other sequences and rows outside never reach a result, whatever they hold. A NaN or infinity in a later row of the SAME sequence
 can reach earlier rows of its tile of 64 under `causal`, as in any matrix product. Head dimensions other than 32, 64 and 128 are padded to the
 next of them (a copy), up to 128. Deterministic; captures into a graph (the offsets may change between replays, the shapes may not). A capture with gradients is refused
@@ -93,14 +94,16 @@ def _forward(q, k, v, table, cu_q, cu_k, causal, scale, buckets, want_stats):
     batch = cu_q.shape[0] - 1
     out = torch.empty((tq, heads, dim), dtype=q.dtype, device=q.device)
     stats = torch.empty((heads, tq, 2), dtype=torch.float32, device=q.device) if want_stats else None
+    rest = torch.empty_like(out) if want_stats and q.dtype != torch.float32 else None      # what the output's rounding leaves over
     n = int(_lib.load().irx_attn_packed_fwd_workspace_bytes(tq, tk, batch, heads, kv_heads, dim, _TYPES[q.dtype], table is not None))
     ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     tb, tb_f32, mp, nb, far = _table_args(table, buckets)
     _lib.call("irx_attn_packed_fwd", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
               v.stride(0), v.stride(1), cu_q.data_ptr(), cu_k.data_ptr(), batch, tq, tk, heads, kv_heads, dim, _TYPES[q.dtype], scale,
-              causal, tb, tb_f32, mp, nb, max(far, 0), out.data_ptr(), stats.data_ptr() if want_stats else None,
+              causal, tb, tb_f32, mp, nb, max(far, 0), out.data_ptr(),
+              rest.data_ptr() if rest is not None else None, stats.data_ptr() if want_stats else None,
               ws.data_ptr() if n else None, n, _lib.stream_ptr())
-    return out, stats
+    return out, stats, rest
 
 
 class AttentionPackedFn(torch.autograd.Function):
@@ -108,15 +111,15 @@ class AttentionPackedFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, table, cu_q, cu_k, causal, scale, buckets):
-        out, stats = _forward(q, k, v, table, cu_q, cu_k, causal, scale, buckets, True)
-        ctx.save_for_backward(q, k, v, table, cu_q, cu_k, buckets, out, stats)
+        out, stats, rest = _forward(q, k, v, table, cu_q, cu_k, causal, scale, buckets, True)
+        ctx.save_for_backward(q, k, v, table, cu_q, cu_k, buckets, out, stats, rest)
         ctx.cfg = (causal, scale)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, table, cu_q, cu_k, buckets, out, stats = ctx.saved_tensors
+        q, k, v, table, cu_q, cu_k, buckets, out, stats, rest = ctx.saved_tensors
         causal, scale = ctx.cfg
         if torch.cuda.is_current_stream_capturing():
             _nodes.refuse_foreign_leaves("attention_packed", _nodes.leaves_of(ctx))
@@ -134,8 +137,8 @@ class AttentionPackedFn(torch.autograd.Function):
         n = int(_lib.load().irx_attn_packed_bwd_workspace_bytes(tq, tk, batch, heads, kv_heads, dim, _TYPES[q.dtype], far))
         ws = torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
         _lib.call("irx_attn_packed_bwd", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                  v.stride(0), v.stride(1), dout.data_ptr(), dout.stride(0), dout.stride(1), out.data_ptr(), stats.data_ptr(),
-                  cu_q.data_ptr(), cu_k.data_ptr(), batch, tq, tk, heads, kv_heads, dim, _TYPES[q.dtype], scale, causal, tb, tb_f32,
+                  v.stride(0), v.stride(1), dout.data_ptr(), dout.stride(0), dout.stride(1), out.data_ptr(),
+                  rest.data_ptr() if rest is not None else None, stats.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), batch, tq, tk, heads, kv_heads, dim, _TYPES[q.dtype], scale, causal, tb, tb_f32,
                   mp, nb, max(far, 0), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dt.data_ptr() if dt is not None else None,
                   ws.data_ptr(), n, _lib.stream_ptr())
         return dq, dk, dv, dt, None, None, None, None, None

@@ -184,12 +184,14 @@ __global__ __launch_bounds__(256, (fwd_waves<T, D>())) void k_attn_fwd(AtParams 
     }
     return;
   }
-  S* o = reinterpret_cast<S*>(P.dst) + ((size_t)q * P.heads + head) * D + 4 * half;
+  const size_t at = ((size_t)q * P.heads + head) * D + 4 * half;
+  S* o = reinterpret_cast<S*>(P.dst) + at;
+  S* rest = P.dst2 ? reinterpret_cast<S*>(P.dst2) + at : nullptr;
 #pragma unroll
   for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
     for (int g = 0; g < 4; ++g)
-      at_st4<T>(o + 32 * b + 8 * g, acc[b][4 * g] * inv, acc[b][4 * g + 1] * inv, acc[b][4 * g + 2] * inv, acc[b][4 * g + 3] * inv);
+      at_st4_rest<T>(o + 32 * b + 8 * g, rest ? rest + 32 * b + 8 * g : nullptr, acc[b][4 * g] * inv, acc[b][4 * g + 1] * inv, acc[b][4 * g + 2] * inv, acc[b][4 * g + 3] * inv);
   if (P.wstats && half == 0) {
     float* st = P.wstats + ((size_t)head * P.tq + q) * 2;
     st[0] = m == -INFINITY ? 0.f : m;
@@ -367,7 +369,9 @@ __global__ __launch_bounds__(256) void k_attn_join(AtParams P) {
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   const size_t head = row / P.tq, q = row % P.tq;
-  at_st4<T>(reinterpret_cast<typename T::S*>(P.dst) + (q * P.heads + head) * D + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  typedef typename T::S S;
+  const size_t at = (q * P.heads + head) * D + d;
+  at_st4_rest<T>(reinterpret_cast<S*>(P.dst) + at, P.dst2 ? reinterpret_cast<S*>(P.dst2) + at : nullptr, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
   if (P.wstats && c == 0) {
     P.wstats[2 * row] = Ms;
     P.wstats[2 * row + 1] = inv;
@@ -466,7 +470,7 @@ extern "C" size_t irx_attn_packed_fwd_workspace_bytes(int tq, int tk, int batch,
 extern "C" int irx_attn_packed_fwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
                                    const void* v, long long v_row, long long v_head, const int32_t* cu_q, const int32_t* cu_k, int batch,
                                    int tq, int tk, int heads, int kv_heads, int dim, int dtype, float scale, int causal, const void* table,
-                                   int table_f32, const int32_t* map, int buckets, int far, void* out, float* stats, void* workspace,
+                                   int table_f32, const int32_t* map, int buckets, int far, void* out, void* rest, float* stats, void* workspace,
                                    size_t workspace_bytes, void* stream) {
   AtParams P = {};
   P.q = {q, q_row, q_head};
@@ -475,10 +479,10 @@ extern "C" int irx_attn_packed_fwd(const void* q, long long q_row, long long q_h
   P.cu_q = cu_q; P.cu_k = cu_k;
   P.batch = batch; P.tq = tq; P.tk = tk; P.heads = heads; P.kv_heads = kv_heads; P.causal = causal != 0; P.scale = scale;
   P.table = table; P.table_f32 = table_f32; P.map = map; P.buckets = buckets; P.far = far;
-  P.dst = out; P.wstats = stats;
+  P.dst = out; P.dst2 = dtype == IRX_ATTN_F32 ? nullptr : rest; P.wstats = stats;
   if (int rc = at_check("irx_attn_packed_fwd", P, dim, dtype, dtype == IRX_ATTN_F32 ? 4 : 2)) return rc;
   if (tq == 0) return IRX_OK;
-  IRX_REQUIRE(out && ((uintptr_t)out & 15) == 0, "irx_attn_packed_fwd: out must be given and start on 16 bytes");
+  IRX_REQUIRE(out && (((uintptr_t)out | (uintptr_t)rest) & 15) == 0, "irx_attn_packed_fwd: out must be given and start on 16 bytes");
   P.slots = at_slots(tq, batch, IRX_ATTN_BM);
   const FwdPlan plan = fwd_plan(tq, tk, batch, heads, kv_heads, dim, dtype == IRX_ATTN_F32 ? 4 : 2, table != nullptr);
   P.splits = plan.splits;

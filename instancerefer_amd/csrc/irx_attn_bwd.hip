@@ -6,7 +6,7 @@
 // owns queries and walks the keys (D, dq, bias gradient), the other owns keys and walks the group's queries (dk, dv). Scores and dout . v
 // are computed in both: 7 products in place of 5. Both use the transposed layouts of irx_attn.h: P and dS are operands as they come.
 // P and dS are rounded to the operand type for the second products; row statistics, D, dS itself and all sums are 32 bits. D is formed
-// from the stored (rounded) output, as the formula's own terms are no more exact than that.
+// from the stored output and what its rounding left over, where the forward kept that.
 #include "irx_attn.h"
 
 #include <type_traits>
@@ -97,13 +97,15 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
     const S* qp = reinterpret_cast<const S*>(P.q.p) + q * P.q.st + head * P.q.sh + 8 * half;
     const S* dp = reinterpret_cast<const S*>(P.dout.p) + q * P.dout.st + head * P.dout.sh + 8 * half;
     const S* op = reinterpret_cast<const S*>(P.out) + ((size_t)q * P.heads + head) * D + 8 * half;
+    const S* rp = reinterpret_cast<const S*>(P.rest) + ((size_t)q * P.heads + head) * D + 8 * half;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
       qf[s] = mine ? at_ldg<T>(qp + 16 * s) : at_zero<T>();
       df[s] = mine ? at_ldg<T>(dp + 16 * s) : at_zero<T>();
       const F of = mine ? at_ldg<T>(op + 16 * s) : at_zero<T>();
+      const F rf = mine && P.rest ? at_ldg<T>(rp + 16 * s) : at_zero<T>();
 #pragma unroll
-      for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(at_get<T>(of, e), at_get<T>(df[s], e), delta);
+      for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(at_get<T>(of, e) + at_get<T>(rf, e), at_get<T>(df[s], e), delta);
     }
     delta = at_pair_sum(delta);
     if (mine) {
@@ -596,7 +598,7 @@ extern "C" size_t irx_attn_packed_bwd_workspace_bytes(int tq, int tk, int batch,
 
 extern "C" int irx_attn_packed_bwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
                                    const void* v, long long v_row, long long v_head, const void* dout, long long do_row, long long do_head,
-                                   const void* out, const float* stats, const int32_t* cu_q, const int32_t* cu_k, int batch, int tq, int tk,
+                                   const void* out, const void* rest, const float* stats, const int32_t* cu_q, const int32_t* cu_k, int batch, int tq, int tk,
                                    int heads, int kv_heads, int dim, int dtype, float scale, int causal, const void* table, int table_f32,
                                    const int32_t* map, int buckets, int far, void* dq, void* dk, void* dv, void* dtable, void* workspace,
                                    size_t workspace_bytes, void* stream) {
@@ -608,12 +610,12 @@ extern "C" int irx_attn_packed_bwd(const void* q, long long q_row, long long q_h
   P.cu_q = cu_q; P.cu_k = cu_k;
   P.batch = batch; P.tq = tq; P.tk = tk; P.heads = heads; P.kv_heads = kv_heads; P.causal = causal != 0; P.scale = scale;
   P.table = table; P.table_f32 = table_f32; P.map = map; P.buckets = buckets; P.far = far;
-  P.out = out; P.stats = stats;
+  P.out = out; P.rest = dtype == IRX_ATTN_F32 ? nullptr : rest; P.stats = stats;
   if (int rc = at_check("irx_attn_packed_bwd", P, dim, dtype, dtype == IRX_ATTN_F32 ? 4 : 2)) return rc;
   IRX_REQUIRE(tq == 0 || (dout && out && stats && dq), "irx_attn_packed_bwd: null tensor");
   IRX_REQUIRE(tk == 0 || (dk && dv), "irx_attn_packed_bwd: null gradient");
   IRX_REQUIRE(!table || dtable, "irx_attn_packed_bwd: null bias gradient");
-  IRX_REQUIRE((((uintptr_t)out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) == 0, "irx_attn_packed_bwd: rows must start on 16 bytes");
+  IRX_REQUIRE((((uintptr_t)out | (uintptr_t)rest | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) == 0, "irx_attn_packed_bwd: rows must start on 16 bytes");
   const size_t need = irx_attn_packed_bwd_workspace_bytes(tq, tk, batch, heads, kv_heads, dim, dtype, table ? far : -1);
   if (need && (!workspace || workspace_bytes < need)) {
     irx_set_error("irx_attn_packed_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);

@@ -37,9 +37,9 @@ namespace {
 
 typedef size_t (*attn_fwd_ws_fn)(int, int, int, int, int, int, int, int);
 typedef int (*attn_fwd_fn)(const void*, ll, ll, const void*, ll, ll, const void*, ll, ll, const int32_t*, const int32_t*, int, int, int, int, int, int,
-                           int, float, int, const void*, int, const int32_t*, int, int, void*, float*, void*, size_t, void*);
+                           int, float, int, const void*, int, const int32_t*, int, int, void*, void*, float*, void*, size_t, void*);
 typedef size_t (*attn_bwd_ws_fn)(int, int, int, int, int, int, int, int);
-typedef int (*attn_bwd_fn)(const void*, ll, ll, const void*, ll, ll, const void*, ll, ll, const void*, ll, ll, const void*, const float*,
+typedef int (*attn_bwd_fn)(const void*, ll, ll, const void*, ll, ll, const void*, ll, ll, const void*, ll, ll, const void*, const void*, const float*,
                            const int32_t*, const int32_t*, int, int, int, int, int, int, int, float, int, const void*, int, const int32_t*, int, int,
                            void*, void*, void*, void*, void*, size_t, void*);
 typedef int (*rms_fwd_fn)(const void*, const void*, const void*, int, ll, int, int, float, void*, void*, float*, void*);
@@ -96,18 +96,21 @@ struct Attn {
   int far() const { return table.defined() ? (int)(map.size(0) - 1) / 2 : -1; }
 };
 
-Tensor attn_forward(const Attn& a, Tensor* stats, void* stream) {
+// stats, rest: what the backward needs of the forward (NULL: no backward)
+Tensor attn_forward(const Attn& a, Tensor* stats, Tensor* rest, void* stream) {
   const Tensor &q = a.q, &k = a.k;
   const int tq = (int)q.size(0), heads = (int)q.size(1), dim = (int)q.size(2), tk = (int)k.size(0), kv = (int)k.size(1);
   Tensor out = at::empty({tq, heads, dim}, q.options());
   if (stats) *stats = at::empty({heads, tq, 2}, q.options().dtype(at::kFloat));
+  if (rest && q.scalar_type() != at::kFloat) *rest = at::empty_like(out);
   const size_t n = g_text.attn_fwd_ws(tq, tk, a.batch(), heads, kv, dim, type_of(q), a.table.defined());
   const Tensor ws = n ? bytes(n, q) : Tensor();
   const bool b = a.table.defined();
   check(g_text.attn_fwd(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), a.v.data_ptr(), a.v.stride(0), a.v.stride(1),
                         a.cu_q.data_ptr<int32_t>(), a.cu_k.data_ptr<int32_t>(), a.batch(), tq, tk, heads, kv, dim, type_of(q), (float)a.scale, a.causal,
                         b ? a.table.data_ptr() : nullptr, b ? a.table.scalar_type() == at::kFloat : 1, b ? a.map.data_ptr<int32_t>() : nullptr,
-                        b ? (int)a.table.size(0) : 0, b ? a.far() : 0, out.data_ptr(), stats ? stats->data_ptr<float>() : nullptr,
+                        b ? (int)a.table.size(0) : 0, b ? a.far() : 0, out.data_ptr(), rest && rest->defined() ? rest->data_ptr() : nullptr,
+                        stats ? stats->data_ptr<float>() : nullptr,
                         n ? ws.data_ptr() : nullptr, n, stream),
         "irx_attn_packed_fwd");
   return out;
@@ -117,8 +120,8 @@ struct AttnNode : public torch::autograd::Function<AttnNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& table, const Tensor& cu_q,
                         const Tensor& cu_k, const OptTensor& map, bool causal, double scale, int64_t stream) {
     Attn a{q, k, v, table.has_value() ? *table : Tensor(), cu_q, cu_k, map.has_value() ? *map : Tensor(), scale, causal};
-    Tensor stats, out = attn_forward(a, &stats, (void*)stream);
-    ctx->save_for_backward({q, k, v, a.table, cu_q, cu_k, a.map, out, stats});
+    Tensor stats, rest, out = attn_forward(a, &stats, &rest, (void*)stream);
+    ctx->save_for_backward({q, k, v, a.table, cu_q, cu_k, a.map, out, stats, rest});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["stream"] = stream;                   // (the engine replays the node on its forward stream)
@@ -128,7 +131,7 @@ struct AttnNode : public torch::autograd::Function<AttnNode> {
   static variable_list backward(AutogradContext* ctx, variable_list grad_out) {
     const auto s = ctx->get_saved_variables();
     Attn a{s[0], s[1], s[2], s[3], s[4], s[5], s[6], ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool()};
-    const Tensor &q = a.q, &k = a.k, &out = s[7], &stats = s[8];
+    const Tensor &q = a.q, &k = a.k, &out = s[7], &stats = s[8], &rest = s[9];
     void* stream = (void*)ctx->saved_data["stream"].toInt();
     if (g_text.capturing(stream)) refuse_foreign(ctx, {q, k, a.v, a.table.defined() ? OptTensor(a.table) : OptTensor()}, "attention_packed");
     const Tensor dout = rows(grad_out[0]);
@@ -140,7 +143,7 @@ struct AttnNode : public torch::autograd::Function<AttnNode> {
     const size_t n = g_text.attn_bwd_ws(tq, tk, a.batch(), heads, kv, dim, type_of(q), a.far());
     const Tensor ws = bytes(n ? n : 16, q);
     check(g_text.attn_bwd(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), a.v.data_ptr(), a.v.stride(0), a.v.stride(1),
-                          dout.data_ptr(), dout.stride(0), dout.stride(1), out.data_ptr(), stats.data_ptr<float>(), a.cu_q.data_ptr<int32_t>(),
+                          dout.data_ptr(), dout.stride(0), dout.stride(1), out.data_ptr(), rest.defined() ? rest.data_ptr() : nullptr, stats.data_ptr<float>(), a.cu_q.data_ptr<int32_t>(),
                           a.cu_k.data_ptr<int32_t>(), a.batch(), tq, tk, heads, kv, dim, type_of(q), (float)a.scale, a.causal,
                           b ? a.table.data_ptr() : nullptr, b ? a.table.scalar_type() == at::kFloat : 1, b ? a.map.data_ptr<int32_t>() : nullptr,
                           b ? (int)a.table.size(0) : 0, b ? a.far() : 0, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), b ? dt.data_ptr() : nullptr,
@@ -161,7 +164,7 @@ Tensor attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, con
     if (g_text.capturing((void*)stream)) refuse_foreign(nullptr, {q, k, v, table}, "attention_packed");
     return AttnNode::apply(q, k, v, table, cu_q, cu_k, map, causal, scale, stream);
   }
-  return attn_forward(Attn{q, k, v, table.has_value() ? *table : Tensor(), cu_q, cu_k, map.has_value() ? *map : Tensor(), scale, causal}, nullptr, (void*)stream);
+  return attn_forward(Attn{q, k, v, table.has_value() ? *table : Tensor(), cu_q, cu_k, map.has_value() ? *map : Tensor(), scale, causal}, nullptr, nullptr, (void*)stream);
 }
 
 void rms_forward(const Tensor& x, const Tensor& r, const Tensor& w, double eps, Tensor* y, Tensor* h, Tensor* rstd, void* stream) {

@@ -52,6 +52,7 @@ def reference(q, k, v, cu_q, cu_k, dout=None, causal=False, scale=None, table=No
             O = P @ V
             A = P @ V.abs()
             EO = (E + up + (lk + 8) * U32) * A + HALF[dt] * O.abs() + low
+            ED = (E + up + (lk + 8) * U32) * A + HALF[dt] ** 2 * O.abs() + low       # ... with what the rounding left over added back
             o[r0:r1, h], eo[r0:r1, h] = O, EO
             if dout is None:
                 continue
@@ -59,7 +60,7 @@ def reference(q, k, v, cu_q, cu_k, dout=None, causal=False, scale=None, table=No
             dP = G @ V.t()
             D = (G * O).sum(1, keepdim=True)
             S = P * (dP - D)
-            eS = E * S.abs() + P * ((dim + 4) * U32 * (G.abs() @ V.abs().t()) + (G.abs() * EO).sum(1, keepdim=True)
+            eS = E * S.abs() + P * ((dim + 4) * U32 * (G.abs() @ V.abs().t()) + (G.abs() * (EO if dt == torch.float32 else ED)).sum(1, keepdim=True)
                                     + (dim + 4) * U32 * (G.abs() * O.abs()).sum(1, keepdim=True)) + 4 * U32 * S.abs()
             eR = eS + up * S.abs() + sub
             g["dq"][r0:r1, h] = scale * (S @ K)

@@ -110,7 +110,7 @@ def test_c_entries_refuse(lib):
     one = ctypes.c_void_p(4096)
 
     def call(dim=64, dtype=0, heads=4, kv=2, scale=0.1, q=one, row=256, far=0, table=None, tq=8, out=one, cu=one):
-        return f(q, row, 64, one, 128, 64, one, 128, 64, cu, cu, 1, tq, 8, heads, kv, dim, dtype, scale, 0, table, 1, one, 4, far, out, None, None, 0, None)
+        return f(q, row, 64, one, 128, 64, one, 128, 64, cu, cu, 1, tq, 8, heads, kv, dim, dtype, scale, 0, table, 1, one, 4, far, out, None, None, None, 0, None)
 
     for kw in (dict(dim=48), dict(dtype=3), dict(heads=3), dict(kv=0), dict(scale=0.0), dict(scale=math.nan), dict(scale=math.inf), dict(q=ctypes.c_void_p(4100)),
                dict(row=257), dict(table=one, far=A.MAX_FAR + 1), dict(table=one, far=-1), dict(tq=-1), dict(out=None), dict(cu=None), dict(q=None)):
@@ -120,10 +120,10 @@ def test_c_entries_refuse(lib):
     assert lib.irx_attn_packed_fwd_workspace_bytes(16, 16, 1, 4, 4, 64, 0, 0) == 0
     need = lib.irx_attn_packed_fwd_workspace_bytes(1, 8000, 1, 4, 2, 64, 0, 0)
     assert need > 0 and need % ((64 + 2) * 4 * 4) == 0
-    assert f(one, 256, 64, one, 128, 64, one, 128, 64, one, one, 1, 1, 8000, 4, 2, 64, 0, 0.1, 0, None, 1, None, 0, 0, one, None, None, 0, None) == -3
+    assert f(one, 256, 64, one, 128, 64, one, 128, 64, one, one, 1, 1, 8000, 4, 2, 64, 0, 0.1, 0, None, 1, None, 0, 0, one, None, None, None, 0, None) == -3
     assert lib.irx_attn_packed_bwd_workspace_bytes(100, 100, 2, 4, 4, 64, 0, -1) == 100 * 4 * 4
     assert lib.irx_attn_packed_bwd_workspace_bytes(100, 100, 2, 4, 4, 64, 0, 8) > 100 * 4 * 4
-    assert lib.irx_attn_packed_bwd(one, 256, 64, one, 128, 64, one, 128, 64, one, 256, 64, one, one, one, one, 1, 8, 8, 4, 2, 64, 0, 0.1, 0, None, 1, None,
+    assert lib.irx_attn_packed_bwd(one, 256, 64, one, 128, 64, one, 128, 64, one, 256, 64, one, None, one, one, one, 1, 8, 8, 4, 2, 64, 0, 0.1, 0, None, 1, None,
                                    0, 0, one, one, one, None, None, 0, None) == -3
     assert lib.irx_rms_norm_fwd(one, None, one, 1, 4, 0, 0, 1e-6, one, None, None, None) == -1
     assert lib.irx_rms_norm_fwd(one, one, one, 1, 4, 8, 0, 1e-6, one, None, None, None) == -1
