@@ -120,8 +120,8 @@ template <int ID> __device__ __forceinline__ double clip_range(const void* p, si
   if (wide) {                                // lo is a multiple of 8
     constexpr int N = ID == 0 ? 4 : 8;
     const size_t end = lo + (hi - lo) / N * N;
-    for (i = lo + (size_t)threadIdx.x * N; i < end; i += 256 * N) {
-      const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const char*>(p) + i * (ID == 0 ? 4 : 2));
+    auto at = [&](size_t k) __attribute__((always_inline)) { return *reinterpret_cast<const uint4*>(static_cast<const char*>(p) + k * (ID == 0 ? 4 : 2)); };
+    auto take = [&](const uint4& u) __attribute__((always_inline)) {
       const unsigned w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -132,7 +132,17 @@ template <int ID> __device__ __forceinline__ double clip_range(const void* p, si
           clip_take(a[e], clip_get<ID>(s, 1), inf);
         }
       }
+    };
+    constexpr size_t ONE = 256 * N;
+    i = lo + (size_t)threadIdx.x * N;
+    for (; i + 3 * ONE < end; i += 4 * ONE) {                            // four loads on their way at a time
+      const uint4 u0 = at(i), u1 = at(i + ONE), u2 = at(i + 2 * ONE), u3 = at(i + 3 * ONE);
+      take(u0);
+      take(u1);
+      take(u2);
+      take(u3);
     }
+    for (; i < end; i += ONE) take(at(i));
     i = end;
   }
   for (i += threadIdx.x; i < hi; i += 256) clip_take(a[0], clip_get<ID>(p, i), inf);
@@ -393,14 +403,23 @@ __global__ __launch_bounds__(256) void k_gather_norm(GatherTable T, unsigned lon
   size_t i = lo;
   if (((((uintptr_t)src) | ((uintptr_t)dst)) & 15) == 0) {
     const size_t end = lo + (hi - lo) / 4 * 4;
-    for (i = lo + (size_t)threadIdx.x * 4; i < end; i += 1024) {
-      const float4 v = *reinterpret_cast<const float4*>(src + i);
-      if (copy) *reinterpret_cast<float4*>(dst + i) = v;
+    auto take = [&](size_t k, const float4& v) __attribute__((always_inline)) {
+      if (copy) *reinterpret_cast<float4*>(dst + k) = v;
       clip_take(a[0], v.x, inf);
       clip_take(a[1], v.y, inf);
       clip_take(a[2], v.z, inf);
       clip_take(a[3], v.w, inf);
+    };
+    auto at = [&](size_t k) __attribute__((always_inline)) { return *reinterpret_cast<const float4*>(src + k); };
+    i = lo + (size_t)threadIdx.x * 4;
+    for (; i + 3072 < end; i += 4096) {                                  // four loads on their way at a time
+      const float4 v0 = at(i), v1 = at(i + 1024), v2 = at(i + 2048), v3 = at(i + 3072);
+      take(i, v0);
+      take(i + 1024, v1);
+      take(i + 2048, v2);
+      take(i + 3072, v3);
     }
+    for (; i < end; i += 1024) take(i, at(i));
     i = end;
   }
   for (i += threadIdx.x; i < hi; i += 256) {
