@@ -514,9 +514,9 @@ __global__ __launch_bounds__(256) void k_attn_dbias(const float* part, int slots
   const int c = count;
   double s = 0;
   if (c) {
-    const int n = slots * c;                                             // slots < 2^25 / heads, c <= 1025
+    const long long n = (long long)slots * c;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < n; i += 256) s += (double)part[((size_t)(i / c) * heads + head) * W + list[i % c]];
+    for (long long i = threadIdx.x; i < n; i += 256) s += (double)part[((size_t)(i / c) * heads + head) * W + list[i % c]];
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);

@@ -127,6 +127,11 @@ def test_rows_outside_every_sequence_and_other_sequences_never_matter(kind, caus
         rows = want[n].shape[0]
         assert torch.equal(got[n][:rows], want[n]), n
         assert float(got[n][rows:].float().abs().max()) == 0.0, n
+    # rows in front of the first sequence
+    front = lambda t: torch.cat((torch.full((5,) + t.shape[1:], math.nan).to(t.dtype), t))  # noqa: E731
+    got = run(front(q), front(k), front(v), cu + 5, cu + 5, front(do), causal)
+    for n in want:
+        assert torch.equal(got[n][5:], want[n]) and float(got[n][:5].float().abs().max()) == 0.0, n
     # a neighbour of infinities
     k2, v2 = k.clone(), v.clone()
     k2[50:51], v2[50:51] = math.inf, math.nan
@@ -259,6 +264,46 @@ def test_rows_beyond_32_bit_offsets():
     assert torch.equal(o, o2) and all(torch.equal(x, y) for x, y in zip(want, got))
 
 
+def test_a_captured_few_query_launch():
+    from instancerefer_amd.attention import attention_packed
+    q, k, v, _ = (t.to(DEV) for t in make([1, 1, 2], [900, 3000, 700], 8, 2, 128, torch.bfloat16, 81))
+    cu, cuk = offsets([1, 1, 2]).to(DEV), offsets([900, 3000, 700]).to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attention_packed(q, k, v, cu, cuk)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = attention_packed(q, k, v, cu, cuk)
+    for ends in ([900, 3000, 700], [4600, 0, 0], [1, 2, 3]):
+        cuk.copy_(offsets(ends))
+        want = attention_packed(q, k, v, cu, cuk)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, want)
+        q.mul_(0.7)
+
+
+def test_two_calls_at_once_on_two_streams():
+    from instancerefer_amd.attention import attention_packed
+    sets = [make([700, 300], [700, 300], 4, 2, 64, torch.bfloat16, s) for s in (91, 92)]
+    sets = [[t.to(DEV) for t in s] for s in sets]
+    cu = offsets([700, 300]).to(DEV)
+    want = [attention_packed(*s[:3], cu, causal=True) for s in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for n in range(2):
+            with torch.cuda.stream(streams[n]):
+                got[n].append(attention_packed(*sets[n][:3], cu, causal=True))
+    torch.cuda.synchronize()
+    for n in range(2):
+        assert all(torch.equal(x, want[n]) for x in got[n])
+
+
 def test_same_bits_every_time_and_on_another_stream():
     from instancerefer_amd.attention import relative_buckets
     lens = [300, 64, 111]
@@ -276,14 +321,15 @@ def test_same_bits_every_time_and_on_another_stream():
             assert torch.equal(got[name], want[name]), name
 
 
-def test_captured_forward_and_backward_with_new_offsets(backend):
+@pytest.mark.parametrize("kind,dim,far", [("bf16", 64, 40), ("f32", 128, 512), ("f16", 128, 512)])      # up to 160 KB of LDS
+def test_captured_forward_and_backward_with_new_offsets(backend, kind, dim, far):
     from instancerefer_amd.attention import attention_packed, relative_buckets
-    dt, total = torch.bfloat16, 260
+    dt, total = TYPES[kind], 260
     g = torch.Generator().manual_seed(6)
-    q, k, v = ((torch.randn(total, h, 64, generator=g)).to(dt).to(DEV).requires_grad_(True) for h in (4, 2, 2))
-    do = torch.randn(total, 4, 64, generator=g).to(dt).to(DEV)
+    q, k, v = ((torch.randn(total, h, dim, generator=g)).to(dt).to(DEV).requires_grad_(True) for h in (4, 2, 2))
+    do = torch.randn(total, 4, dim, generator=g).to(dt).to(DEV)
     table = torch.randn(16, 4, generator=g).to(DEV).requires_grad_(True)
-    buckets = relative_buckets(16, 40, False, device=DEV)
+    buckets = relative_buckets(16, far, False, device=DEV)
     cu = offsets([100, 60, 100]).to(DEV)
     leaves = [q, k, v, table]
 
