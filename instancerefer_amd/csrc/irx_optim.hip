@@ -69,6 +69,8 @@ extern "C" int irx_adam_step(float* params, const float* grads, float* exp_avg, 
 // tensors, in one more read and write that is left out when the factor is 1. Squares are summed in 64 bits (no overflow at 1.8e19, and the
 // double rate is far above what memory delivers): a sum per workgroup, and every workgroup that needs the norm adds those sums itself,
 // in the same order — no atomics, no launch in between.
+// Measured: 60 M values of mixed types (180 MB): sums 35 us (5.1 TB/s; with one load at a time 51), scaling 56 us (6.4 TB/s); 8 M values in
+// 167 tensors: gathered and summed in 20 us (two launches; torch's multi-tensor copy alone 86), Adam with the factor 36 us (6.2 TB/s).
 
 #define IRX_CLIP_TENSORS 160                 // tensors of one launch: the table travels in the kernel's arguments (3.4 of 4 KB)
 #define IRX_CLIP_PARTS 1024                  // wanted number of workgroups
