@@ -519,8 +519,13 @@ __global__ __launch_bounds__(256) void k_attn_dbias(const float* part, int slots
   double s = 0;
   if (c) {
     const long long n = (long long)slots * c;
+    const long long step = (1 << 30) / c * (long long)c;                 // whole tiles at a time, so that the divisions below are 32 bits
+    for (long long from = 0; from < n; from += step) {
+      const float* p0 = part + (size_t)(from / c) * heads * W;
+      const int m = (int)(n - from < step ? n - from : step);
 #pragma unroll 4
-    for (long long i = threadIdx.x; i < n; i += 256) s += (double)part[((size_t)(i / c) * heads + head) * W + list[i % c]];
+      for (int i = threadIdx.x; i < m; i += 256) s += (double)p0[((size_t)(i / c) * heads + head) * W + list[i % c]];
+    }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
