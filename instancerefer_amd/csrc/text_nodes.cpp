@@ -171,8 +171,9 @@ Tensor attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, con
 void rms_forward(const Tensor& x, const Tensor& r, const Tensor& w, double eps, Tensor* y, Tensor* h, Tensor* rstd, void* stream) {
   *y = at::empty_like(x);
   if (r.defined()) *h = at::empty_like(x);
-  if (rstd) *rstd = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
-  check(g_text.rms_fwd(x.data_ptr(), r.defined() ? r.data_ptr() : nullptr, w.data_ptr(), w.scalar_type() == at::kFloat, x.size(0), (int)x.size(1), type_of(x),
+  const int64_t cols = x.size(-1), rows = x.numel() / cols;
+  if (rstd) *rstd = at::empty({rows}, x.options().dtype(at::kFloat));
+  check(g_text.rms_fwd(x.data_ptr(), r.defined() ? r.data_ptr() : nullptr, w.data_ptr(), w.scalar_type() == at::kFloat, rows, (int)cols, type_of(x),
                        (float)eps, y->data_ptr(), h->defined() ? h->data_ptr() : nullptr, rstd ? rstd->data_ptr<float>() : nullptr, stream),
         "irx_rms_norm_fwd");
 }
@@ -199,10 +200,11 @@ struct RmsNode : public torch::autograd::Function<RmsNode> {
     if (g_text.capturing(stream)) refuse_foreign(ctx, {s[3], r.defined() ? OptTensor(r) : OptTensor(), w}, "rms_norm_residual");
     const Tensor dy = grad_out[0].defined() ? grad_out[0].contiguous() : at::zeros_like(h);
     Tensor dx = at::empty_like(h), dw = at::empty_like(w);
-    const size_t n = g_text.rms_bwd_ws(h.size(0), (int)h.size(1), type_of(h));
+    const int64_t cols = h.size(-1), rows = h.numel() / cols;
+    const size_t n = g_text.rms_bwd_ws(rows, (int)cols, type_of(h));
     const Tensor ws = bytes(n, h);
     check(g_text.rms_bwd(dy.data_ptr(), dh.defined() ? dh.data_ptr() : nullptr, h.data_ptr(), w.data_ptr(), w.scalar_type() == at::kFloat, rstd.data_ptr<float>(),
-                         h.size(0), (int)h.size(1), type_of(h), dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), n, stream),
+                         rows, (int)cols, type_of(h), dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), n, stream),
           "irx_rms_norm_bwd");
     variable_list d = once({dx, dw}, "rms_norm_residual");
     g[0] = d[0];
@@ -212,7 +214,7 @@ struct RmsNode : public torch::autograd::Function<RmsNode> {
   }
 };
 
-// x, residual (rows, C) contiguous, weight (C,) contiguous, as rms_norm_residual has checked them -> [y, h] or [y]
+// x, residual (..., C) contiguous, weight (C,) contiguous, as rms_norm_residual has checked them -> [y, h] or [y]
 std::vector<Tensor> rms_norm(const Tensor& x, const OptTensor& r, const Tensor& w, double eps, int64_t stream) {
   if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (r.has_value() && r->requires_grad()))) {
     if (g_text.capturing((void*)stream)) refuse_foreign(nullptr, {x, r, w}, "rms_norm_residual");

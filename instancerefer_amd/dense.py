@@ -537,16 +537,17 @@ def rms_norm_residual(x, residual, weight, eps=1e-6):
     if x.device.index != torch.cuda.current_device():
         with torch.cuda.device(x.device):
             return rms_norm_residual(x, residual, weight, eps)
-    shape = x.shape
-    x2 = x.contiguous().view(-1, shape[-1])
-    r2 = None if residual is None else residual.contiguous().view(-1, shape[-1])
-    weight = weight.contiguous()
+    x, weight = x.contiguous(), weight.contiguous()
+    r = None if residual is None else residual.contiguous()
     if NORM_BACKEND != "py":
         from . import _nodes
         nodes = _nodes.load()
         if nodes is not None:
-            out = nodes.rms_norm(x2, r2, weight, eps, _lib.stream_ptr())
-            return out[0].view(shape), x if r2 is None else out[1].view(shape)
+            out = nodes.rms_norm(x, r, weight, eps, _lib.stream_ptr())         # any number of axes: no view nodes around it
+            return out[0], x if r is None else out[1]
+    shape = x.shape
+    x2 = x.view(-1, shape[-1])
+    r2 = None if r is None else r.view(-1, shape[-1])
     if torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad or (r2 is not None and r2.requires_grad)):
         if torch.cuda.is_current_stream_capturing():
             from . import _nodes
