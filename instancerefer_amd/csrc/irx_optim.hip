@@ -414,12 +414,12 @@ __global__ __launch_bounds__(256) void k_gather_norm(GatherTable T, unsigned lon
     };
     auto at = [&](size_t k) __attribute__((always_inline)) { return *reinterpret_cast<const float4*>(src + k); };
     i = lo + (size_t)threadIdx.x * 4;
-    for (; i + 3072 < end; i += 4096) {                                  // four loads on their way at a time
-      const float4 v0 = at(i), v1 = at(i + 1024), v2 = at(i + 2048), v3 = at(i + 3072);
+    for (; i + 3 * 1024 < end; i += 4 * 1024) {                                  // four loads on their way at a time
+      const float4 v0 = at(i), v1 = at(i + 1024), v2 = at(i + 2 * 1024), v3 = at(i + 3 * 1024);
       take(i, v0);
       take(i + 1024, v1);
-      take(i + 2048, v2);
-      take(i + 3072, v3);
+      take(i + 2 * 1024, v2);
+      take(i + 3 * 1024, v3);
     }
     for (; i < end; i += 1024) take(i, at(i));
     i = end;

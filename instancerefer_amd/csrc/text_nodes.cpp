@@ -226,6 +226,24 @@ std::vector<Tensor> rms_norm(const Tensor& x, const OptTensor& r, const Tensor& 
   return {y};
 }
 
+// The addresses of the gradients of `params` to out (an array of pointers), for the copy that sums their norm. False, with `out` in no
+// certain state, if one of them is no dense contiguous float32 tensor of its own size on the device, or if one of `filled` (parameters whose
+// gradient a producer has delivered already) has a gradient besides: the caller then goes through them one by one.
+bool grad_addresses(const std::vector<Tensor>& params, const std::vector<Tensor>& filled, int64_t device, int64_t counts, int64_t out) {
+  const unsigned long long* n = (const unsigned long long*)counts;
+  void** at = (void**)out;
+  for (const Tensor& p : filled)
+    if (p.grad().defined()) return false;
+  for (size_t i = 0; i < params.size(); ++i) {
+    const Tensor& g = params[i].grad();
+    if (!g.defined() || g.layout() != at::kStrided || g.scalar_type() != at::kFloat || !g.is_cuda() || g.get_device() != device ||
+        (unsigned long long)g.numel() != n[i] || !g.is_contiguous())
+      return false;
+    at[i] = g.data_ptr();
+  }
+  return true;
+}
+
 void bind_text(const std::unordered_map<std::string, int64_t>& p) {
   auto get = [&](const char* n) {
     const auto it = p.find(n);
@@ -249,6 +267,7 @@ void register_text(pybind11::module& m) {
   m.def("bind_text", &bind_text);
   m.def("attention", &attention);
   m.def("rms_norm", &rms_norm);
+  m.def("grad_addresses", &grad_addresses);
 }
 
 }  // namespace irxn

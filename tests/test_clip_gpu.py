@@ -214,6 +214,30 @@ def test_gather_of_gradients_of_every_layout_and_of_many_tensors():
         assert float((a.flat_p - b.flat_p).abs().max()) <= 1e-2 * 64 * 2.0 ** -24 + 2.0 ** -23 * float(a.flat_p.abs().max())
 
 
+def test_addresses_read_at_once_or_one_by_one(monkeypatch):
+    """the same bits either way; a slot that a producer has filled, and one that has a gradient besides, count once"""
+    from instancerefer_amd.optim import FlatAdam
+    pair = [params_of(SHAPES, 8), params_of(SHAPES, 8)]
+    a, b = (FlatAdam(ps, lr=1e-2) for ps in pair)
+    monkeypatch.setattr(b, "_gather_plain", lambda todo, inf_norm: None)
+    for step, (filled, besides) in enumerate([((), ()), ((1,), ()), ((1, 3), (3,)), ((), ())]):
+        g = torch.Generator().manual_seed(step)
+        grads = [torch.randn(p.shape, generator=g).to(DEV) for p in pair[0]]
+        for opt, ps in ((a, pair[0]), (b, pair[1])):
+            opt.zero_grad()
+            for i, p in enumerate(ps):
+                if i in filled:
+                    opt._slots[i].copy_(grads[i])
+                p.grad = grads[i].clone() if i not in filled or i in besides else None
+            if filled:                                                  # as a producer of that group reports it
+                opt._direct.update(filled)
+                opt._direct_groups.add(("group",) + filled)
+        norms = [float(opt.backward_step(max_norm=0.5)) for opt in (a, b)]
+        want = torch.cat([(x * (2 if i in besides else 1)).double().reshape(-1) for i, x in enumerate(grads)])
+        assert abs(norms[0] - float(want.norm())) <= 2 * 2.0 ** -24 * norms[0]
+        assert norms[0] == norms[1] and torch.equal(a.flat_g, b.flat_g) and torch.equal(a.flat_p, b.flat_p)
+
+
 def test_norm_counts_the_mean_over_ranks():
     from instancerefer_amd.optim import FlatAdam
     ps = params_of([(50,)], 4)
