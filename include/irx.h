@@ -631,7 +631,7 @@ int irx_adam_step_clip(float* params, const float* grads, float* exp_avg, float*
  *   fwd: h = x + residual rounded to the type (residual NULL: h is x and is not written), rstd = 1 / sqrt(mean(h^2) + eps) over cols,
  *        y = h * rstd * weight. rstd float32 [rows] (may be NULL).
  *   bwd: dx = dh + rstd * (weight * dy - h rstd * mean(weight * dy * h rstd)) (dh NULL: 0) — the gradient of x and of the residual —
- *        and dweight = sum over rows of dy * h rstd. dx may be dh. Deterministic. rows < 2^31, any cols. */
+ *        and dweight = sum over rows of dy * h rstd. dx may be dh. Deterministic. rows < 2^31, cols < 2^26. */
 int irx_rms_norm_fwd(const void* x, const void* residual, const void* weight, int weight_f32, long long rows, int cols, int dtype,
                      float eps, void* y, void* h, float* rstd, void* stream);
 size_t irx_rms_norm_bwd_workspace_bytes(long long rows, int cols, int dtype);

@@ -7,6 +7,8 @@ import ctypes
 import importlib.util
 import os
 
+import torch
+
 from . import _build, _lib
 
 ENABLED = os.environ.get("IRX_CPP_NODES", "1") != "0"
@@ -77,6 +79,12 @@ def refuse_foreign_leaves(who, leaves):
     if i >= 0:
         raise RuntimeError("%s: a backward pass cannot be captured while an eager graph of the same leaves lives (input %d was used on "
                            "another stream): drop that graph's outputs first, or run the warm-up on the capture's stream" % (who, i))
+
+
+def refuse_capture_of_copies(who, tensors):
+    """refuse_foreign_leaves for an operator that copies its inputs before its node sees them"""
+    if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing() and any(t is not None and t.requires_grad for t in tensors):
+        refuse_foreign_leaves(who, tensors)
 
 
 def leaves_of(ctx):

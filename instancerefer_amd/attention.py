@@ -200,18 +200,20 @@ def attention_packed(q, k, v, cu_q, cu_k=None, causal=False, scale=None, bias=No
         with torch.cuda.device(q.device):
             return attention_packed(q, k, v, cu_q, cu_k, causal, scale, bias, buckets)
     if dim not in _DIMS:
+        _nodes.refuse_capture_of_copies("attention_packed", (q, k, v))
         more = next(d for d in _DIMS if d > dim) - dim
         q, k, v = (torch.nn.functional.pad(t, (0, more)) for t in (q, k, v))
         return attention_packed(q, k, v, cu_q, cu_k, causal, scale, bias, buckets)[..., :dim]
     nodes = _nodes.load() if BACKEND != "py" else None
     if nodes is not None:
         return nodes.attention(q, k, v, bias, cu_q, cu_k, buckets, bool(causal), scale, _lib.stream_ptr())
+    leaves = (q, k, v, bias)
     q, k, v = _rows(q), _rows(k), _rows(v)
     if bias is not None:
         bias = bias.contiguous()
     causal = 1 if causal else 0
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)):
         if torch.cuda.is_current_stream_capturing():
-            _nodes.refuse_foreign_leaves("attention_packed", (q, k, v, bias))
+            _nodes.refuse_foreign_leaves("attention_packed", leaves)
         return AttentionPackedFn.apply(q, k, v, bias, cu_q, cu_k, causal, scale, buckets)
     return _forward(q, k, v, bias, cu_q, cu_k, causal, scale, buckets, False)[0]

@@ -300,6 +300,7 @@ extern "C" size_t irx_rms_norm_bwd_workspace_bytes(long long rows, int cols, int
 
 template <int ID, int N> static void rms_launch_fwd(const RmsForm& f, const void* x, const void* r, const void* w, int wf, long long rows, int cols, float eps,
                                                     void* y, void* h, float* rstd, hipStream_t st) {
+  // (a launch holds fewer than 2^32 threads: the wrapper below hands over at most 2^22 workgroups' rows at a time)
   const unsigned grid = (unsigned)((rows + 256 / f.g - 1) / (256 / f.g));
 #define IRX_RMS(G_, NV_) k_rms_fwd<ID, N, G_, NV_><<<grid, 256, 0, st>>>(x, r, w, wf, rows, cols, eps, y, h, rstd)
   if constexpr (N == 1) IRX_RMS(256, 0);
@@ -326,7 +327,7 @@ template <int ID, int N> static void rms_launch_bwd(const RmsForm& f, int groups
 
 static int rms_check(const char* who, long long rows, int cols, int dtype, const void* a, const void* b, const void* c, const void* d) {
   IRX_REQUIRE(dtype >= 0 && dtype <= 2, "%s: type %d (0 float32, 1 bfloat16, 2 float16)", who, dtype);
-  IRX_REQUIRE(rows >= 0 && rows < (1ll << 31) && cols >= 1, "%s: %lld rows of %d", who, rows, cols);
+  IRX_REQUIRE(rows >= 0 && rows < (1ll << 31) && cols >= 1 && cols < (1 << 26), "%s: %lld rows of %d", who, rows, cols);
   IRX_REQUIRE(rows == 0 || (a && b && c && d), "%s: null tensor", who);
   return IRX_OK;
 }
@@ -339,9 +340,18 @@ extern "C" int irx_rms_norm_fwd(const void* x, const void* residual, const void*
   if (rows == 0) return IRX_OK;
   const RmsForm f = rms_form(cols, dtype, al16(x) && al16(residual) && al16(weight) && al16(y) && al16(h));
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == 0) f.n == 1 ? rms_launch_fwd<0, 1>(f, x, residual, weight, 1, rows, cols, eps, y, h, rstd, st) : rms_launch_fwd<0, 4>(f, x, residual, weight, 1, rows, cols, eps, y, h, rstd, st);
-  else if (dtype == 1) f.n == 1 ? rms_launch_fwd<1, 1>(f, x, residual, weight, weight_f32, rows, cols, eps, y, h, rstd, st) : rms_launch_fwd<1, 8>(f, x, residual, weight, weight_f32, rows, cols, eps, y, h, rstd, st);
-  else f.n == 1 ? rms_launch_fwd<2, 1>(f, x, residual, weight, weight_f32, rows, cols, eps, y, h, rstd, st) : rms_launch_fwd<2, 8>(f, x, residual, weight, weight_f32, rows, cols, eps, y, h, rstd, st);
+  const long long step = (long long)(256 / f.g) << 22;
+  const size_t elem = dtype == 0 ? 4 : 2;
+  for (long long r0 = 0; r0 < rows; r0 += step) {
+    const long long n = rows - r0 < step ? rows - r0 : step;
+    auto from = [&](const void* p) { return p ? static_cast<const char*>(p) + (size_t)r0 * cols * elem : nullptr; };
+    const void *xs = from(x), *rs = from(residual);
+    void *ys = const_cast<char*>(from(y)), *hs = const_cast<char*>(from(h));
+    float* sd = rstd ? rstd + r0 : nullptr;
+    if (dtype == 0) f.n == 1 ? rms_launch_fwd<0, 1>(f, xs, rs, weight, 1, n, cols, eps, ys, hs, sd, st) : rms_launch_fwd<0, 4>(f, xs, rs, weight, 1, n, cols, eps, ys, hs, sd, st);
+    else if (dtype == 1) f.n == 1 ? rms_launch_fwd<1, 1>(f, xs, rs, weight, weight_f32, n, cols, eps, ys, hs, sd, st) : rms_launch_fwd<1, 8>(f, xs, rs, weight, weight_f32, n, cols, eps, ys, hs, sd, st);
+    else f.n == 1 ? rms_launch_fwd<2, 1>(f, xs, rs, weight, weight_f32, n, cols, eps, ys, hs, sd, st) : rms_launch_fwd<2, 8>(f, xs, rs, weight, weight_f32, n, cols, eps, ys, hs, sd, st);
+  }
   IRX_CHECK_LAUNCH("irx_rms_norm_fwd");
   return IRX_OK;
 }

@@ -159,10 +159,10 @@ struct AttnNode : public torch::autograd::Function<AttnNode> {
 // q, k, v, table, offsets and map as attention_packed has checked them
 Tensor attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const OptTensor& table_in, const Tensor& cu_q, const Tensor& cu_k,
                  const OptTensor& map, bool causal, double scale, int64_t stream) {
-  const Tensor q = rows(q_in), k = rows(k_in), v = rows(v_in);
+  const Tensor q = rows(q_in), k = rows(k_in), v = rows(v_in);           // (a copy of a leaf leads back to it: the leaves themselves are asked)
   const OptTensor table = table_in.has_value() ? OptTensor(table_in->contiguous()) : table_in;
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (table.has_value() && table->requires_grad()))) {
-    if (g_text.capturing((void*)stream)) refuse_foreign(nullptr, {q, k, v, table}, "attention_packed");
+    if (g_text.capturing((void*)stream)) refuse_foreign(nullptr, {q_in, k_in, v_in, table_in}, "attention_packed");
     return AttnNode::apply(q, k, v, table, cu_q, cu_k, map, causal, scale, stream);
   }
   return attn_forward(Attn{q, k, v, table.has_value() ? *table : Tensor(), cu_q, cu_k, map.has_value() ? *map : Tensor(), scale, causal}, nullptr, nullptr, (void*)stream);

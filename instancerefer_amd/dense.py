@@ -520,8 +520,8 @@ def rms_norm_residual(x, residual, weight, eps=1e-6):
 
     x, residual (..., C) float32, bfloat16 or float16; weight (C,) float32 or x's type. Differentiable in all three (once); the gradient
     with respect to h (what the later blocks send back) joins the norm's in the same launch."""
-    if x.dim() < 1 or x.shape[-1] < 1 or x.dtype not in _NORM_TYPES:
-        raise ValueError("rms_norm_residual: x must be (..., C) in float32, bfloat16 or float16, got %s of %s" % (tuple(x.shape), x.dtype))
+    if x.dim() < 1 or not 1 <= x.shape[-1] < 1 << 26 or x.dtype not in _NORM_TYPES:
+        raise ValueError("rms_norm_residual: x must be (..., C), C below 2^26, in float32, bfloat16 or float16, got %s of %s" % (tuple(x.shape), x.dtype))
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError("rms_norm_residual: x is %s of %s, the residual %s of %s" % (tuple(x.shape), x.dtype, tuple(residual.shape), residual.dtype))
     if weight.shape != x.shape[-1:] or weight.dtype not in (_f32, x.dtype):
@@ -537,21 +537,23 @@ def rms_norm_residual(x, residual, weight, eps=1e-6):
     if x.device.index != torch.cuda.current_device():
         with torch.cuda.device(x.device):
             return rms_norm_residual(x, residual, weight, eps)
-    x, weight = x.contiguous(), weight.contiguous()
-    r = None if residual is None else residual.contiguous()
+    xc, wc, r = x.contiguous(), weight.contiguous(), None if residual is None else residual.contiguous()
+    if xc is not x or wc is not weight or r is not residual:
+        from . import _nodes
+        _nodes.refuse_capture_of_copies("rms_norm_residual", (x, residual, weight))
     if NORM_BACKEND != "py":
         from . import _nodes
         nodes = _nodes.load()
         if nodes is not None:
-            out = nodes.rms_norm(x, r, weight, eps, _lib.stream_ptr())         # any number of axes: no view nodes around it
+            out = nodes.rms_norm(xc, r, wc, eps, _lib.stream_ptr())            # any number of axes: no view nodes around it
             return out[0], x if r is None else out[1]
-    shape = x.shape
-    x2 = x.view(-1, shape[-1])
+    shape, weight = x.shape, wc
+    x2 = xc.view(-1, shape[-1])
     r2 = None if r is None else r.view(-1, shape[-1])
     if torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad or (r2 is not None and r2.requires_grad)):
         if torch.cuda.is_current_stream_capturing():
             from . import _nodes
-            _nodes.refuse_foreign_leaves("rms_norm_residual", (x2, r2, weight))
+            _nodes.refuse_foreign_leaves("rms_norm_residual", (x, residual, weight))
         out = RMSNormFn.apply(x2, r2, weight, eps)
         y, h = (out, None) if r2 is None else out
     else:

@@ -379,6 +379,31 @@ def test_capture_beside_a_living_eager_graph_is_refused(backend):
     assert float(torch.autograd.grad(alive, q, do)[0].abs().max()) > 0
 
 
+@pytest.mark.parametrize("how", ["padded", "copied", "table"])
+def test_capture_beside_a_living_eager_graph_of_copied_leaves(how, backend):
+    """a leaf that the operator pads or copies before its node sees it is found too"""
+    from instancerefer_amd.attention import attention_packed, relative_buckets
+    dim = 40 if how == "padded" else 64
+    q, k, v, do = (t.to(DEV) for t in make([40], [40], 2, 2, dim, torch.float32, 62))
+    cu, args = offsets([40]).to(DEV), {}
+    if how == "copied":
+        buf = torch.empty(q.numel() + 1, device=DEV)[1:]
+        q = buf.copy_(q.reshape(-1)).view(q.shape)
+    if how == "table":
+        leaf = torch.zeros((2, 8), device=DEV).t()                      # (8, 2), not contiguous
+        args = {"bias": leaf, "buckets": relative_buckets(8, 16, device=DEV)}
+    else:
+        leaf = q
+    leaf.requires_grad_(True)
+    alive = attention_packed(q, k, v, cu, **args)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(graph):
+            attention_packed(q, k, v, cu, **args)
+    torch.cuda.synchronize()
+    assert float(torch.autograd.grad(alive, leaf, do)[0].abs().max()) > 0
+
+
 def test_second_derivative_is_refused(backend):
     from instancerefer_amd.attention import attention_packed
     q, k, v, do = (t.to(DEV) for t in make([9], [9], 2, 2, 32, torch.float32, 71))

@@ -161,6 +161,43 @@ def test_captured_and_on_another_stream(backend):
             x.mul_(1.1)
 
 
+@pytest.mark.parametrize("rows,cols,kind", [(2 ** 24 + 5, 1, torch.float32), (2 ** 26 + 3, 8, torch.bfloat16)])
+def test_more_rows_than_one_launch(rows, cols, kind, backend):
+    from instancerefer_amd.dense import rms_norm_residual
+    g = torch.Generator(device=DEV).manual_seed(11)
+    x = torch.randn((rows, cols), generator=g, device=DEV).to(kind)
+    w = torch.linspace(0.5, 1.5, cols, device=DEV)
+    y, h = rms_norm_residual(x, x, w)
+    trained = torch.nn.Parameter(w)                                     # (a call with gradients keeps one more value per row)
+    y2, _ = rms_norm_residual(x, x, trained)
+    assert torch.equal(y, y2.detach())
+    half = torch.finfo(kind).eps / 2
+    for lo in list(range(0, rows, 1 << 22)):
+        xs = x[lo:lo + (1 << 22)].double()
+        assert torch.equal(h[lo:lo + (1 << 22)].double(), 2 * xs)       # doubling is exact
+        want = 2 * xs / (4 * xs.square().mean(1, keepdim=True) + 1e-6).sqrt() * w.double()
+        # sum of 8 squares, the mean, eps, the inverse root (2 half steps) and two products in 32 bits, then the type's rounding
+        assert ((y[lo:lo + (1 << 22)].double() - want).abs() <= (half + 16 * 2.0 ** -24) * want.abs() + 1e-40).all()
+
+
+@pytest.mark.parametrize("leaf", ["x", "x transposed", "residual"])
+def test_capture_beside_a_living_eager_graph_of_other_leaves(leaf, backend):
+    """a leaf that the operator views or copies first is found too"""
+    from instancerefer_amd.dense import rms_norm_residual
+    x, res, w, dy, dh = (t.to(DEV) for t in inputs(6, 64, torch.float32, torch.float32, 12))
+    if leaf == "x transposed":
+        x = x.t().contiguous().t()
+    (res if leaf == "residual" else x).requires_grad_(True)
+    alive = rms_norm_residual(x, res, w)
+    assert rms_norm_residual(x, None, w)[1] is x
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(graph):
+            rms_norm_residual(x, res, w)
+    torch.cuda.synchronize()
+    assert alive[0].requires_grad
+
+
 def test_capture_beside_a_living_eager_graph_is_refused(backend):
     from instancerefer_amd.dense import rms_norm_residual
     x, res, w, dy, dh = (t.to(DEV) for t in inputs(7, 64, torch.float32, torch.float32, 10))

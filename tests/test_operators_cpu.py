@@ -126,6 +126,7 @@ def test_c_entries_refuse(lib):
     assert lib.irx_attn_packed_bwd(one, 256, 64, one, 128, 64, one, 128, 64, one, 256, 64, one, None, one, one, one, 1, 8, 8, 4, 2, 64, 0, 0.1, 0, None, 1, None,
                                    0, 0, one, one, one, None, None, 0, None) == -3
     assert lib.irx_rms_norm_fwd(one, None, one, 1, 4, 0, 0, 1e-6, one, None, None, None) == -1
+    assert lib.irx_rms_norm_fwd(one, None, one, 1, 4, 1 << 26, 0, 1e-6, one, None, None, None) == -1
     assert lib.irx_rms_norm_fwd(one, one, one, 1, 4, 8, 0, 1e-6, one, None, None, None) == -1
     assert lib.irx_rms_norm_fwd(None, None, None, 1, 0, 8, 0, 1e-6, None, None, None, None) == 0
     assert lib.irx_rms_norm_bwd(one, None, one, one, 1, one, 4, 8, 0, one, one, None, 0, None) == -3
