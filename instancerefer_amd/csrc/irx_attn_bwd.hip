@@ -171,10 +171,10 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
         const int lo = k1 - (i0 + 31 + off), hi = k1 + 31 - (i0 + off);
         near = !(hi <= -P.far || lo >= P.far);
         inside = lo > -P.far && hi < P.far;
-        if (!near) {
-          const float b = sb[hi <= -P.far ? 0 : 2 * P.far] - m;
+        if (!near) {                                                     // (never bias - m first: the forward rounds score + bias)
+          const float b = sb[hi <= -P.far ? 0 : 2 * P.far];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) p[i] = at_exp2(__builtin_fmaf(x[i], c1, b)) * inv;
+          for (int i = 0; i < 16; ++i) p[i] = at_exp2(__builtin_fmaf(x[i], c1, b) - m) * inv;
         } else if (inside) {
           const float* b = sb + d0 + P.far;
 #pragma unroll

@@ -114,6 +114,17 @@ def test_position_bias_that_forbids_buckets():
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_lowest_bias_beyond_the_clipped_distance(kind, dim):
+    """every key a row sees is equally forbidden, most of them beyond the clipped distance: the mean, and the mean's gradients"""
+    from instancerefer_amd.attention import relative_buckets
+    table = torch.full((8, 2), torch.finfo(torch.float32).min)
+    compare([40, 1, 130], [200, 170, 400], 2, 1, dim, kind, True, table=table, buckets=relative_buckets(8, 20, False), spread=2.0)
+    table[:7] = -math.inf                      # ... and those within it not allowed at all
+    compare([40, 1, 130], [200, 170, 400], 2, 1, dim, kind, True, table=table, buckets=relative_buckets(8, 20, False), spread=2.0)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("causal", [False, True])
 def test_rows_outside_every_sequence_and_other_sequences_never_matter(kind, causal):
     from instancerefer_amd.attention import attention_packed
