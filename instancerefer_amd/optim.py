@@ -502,7 +502,11 @@ class FlatAdam:
         the ranks; norm_type 2 or inf) is clipped to it first — the factor goes into the Adam launch, flat_g stays as it is. Returns the norm
         before clipping as a 0-dim device tensor (no host read), or None without max_norm."""
         if max_norm is not None:
-            return self._step_clipped(*_clip_args("FlatAdam.step", max_norm, norm_type))
+            args = _clip_args("FlatAdam.step", max_norm, norm_type)
+            if self.device.type == "cuda" and self.device.index != torch.cuda.current_device():
+                with torch.cuda.device(self.device):
+                    return self._step_clipped(*args)
+            return self._step_clipped(*args)
         for lo, hi, step in self._runs():
             _lib.call("irx_adam_step", _lib.ptr(self.flat_p[lo:hi]), _lib.ptr(self.flat_g[lo:hi]),
                       _lib.ptr(self.exp_avg[lo:hi]), _lib.ptr(self.exp_avg_sq[lo:hi]), hi - lo, float(self.lr),
@@ -535,6 +539,9 @@ class FlatAdam:
         """After loss.backward(): gather -> all-reduce -> (clip ->) Adam. Returns what step() returns. With max_norm on one rank the norm
         is summed while the gradients are gathered."""
         if max_norm is not None and self.device.type == "cuda" and not self._multi_rank():
+            if self.device.index != torch.cuda.current_device():
+                with torch.cuda.device(self.device):
+                    return self.backward_step(max_norm, norm_type)
             max_norm, inf_norm = _clip_args("FlatAdam.backward_step", max_norm, norm_type)
             return self._step_clipped(max_norm, inf_norm, self.gather_grads(inf_norm))
         self.gather_grads()
