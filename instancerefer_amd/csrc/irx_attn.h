@@ -52,6 +52,7 @@ struct AtParams {
   const void* table; const int32_t* map;     // bias table [buckets][heads] (float32 or the tensors' type), map [2 far + 1]
   int table_f32, buckets, far;
   float* part;                               // backward: bias gradient by distance, [slots][heads][2 far + 1]
+  void* dtable;                              // ... and by bucket, the result
   int slots;
   int splits; float* so; float* sst;         // forward over a long axis in parts: partial outputs and (max, sum)
 };

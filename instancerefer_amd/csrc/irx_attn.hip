@@ -440,7 +440,9 @@ int at_check(const char* who, const AtParams& P, int dim, int dtype, int elem) {
   }
   const long long rows = P.tq > P.tk ? P.tq : P.tk;
   IRX_REQUIRE(rows + P.batch + 2 < (1ll << 30), "%s: too many rows", who);
-  IRX_REQUIRE((rows / IRX_ATTN_BM + P.batch + 2) * P.heads < (1ll << 24), "%s: too many tiles", who);          // (256 threads each: below 2^32)
+  // (256 threads each, fewer than 2^32 in a launch; the backward's holds a workgroup per value of the bias table besides)
+  IRX_REQUIRE((rows / IRX_ATTN_BM + P.batch + 2) * P.heads < 3ll << 22, "%s: too many tiles", who);
+  IRX_REQUIRE(!P.table || (long long)P.buckets * P.heads < 1ll << 22, "%s: a bias table of %d buckets", who, P.buckets);
   return IRX_OK;
 }
 

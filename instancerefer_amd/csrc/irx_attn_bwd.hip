@@ -257,20 +257,83 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
       at_st4<T>(o + 32 * b + 8 * g, acc[b][4 * g] * P.scale, acc[b][4 * g + 1] * P.scale, acc[b][4 * g + 2] * P.scale, acc[b][4 * g + 3] * P.scale);
 }
 
+// ---- bias gradient: distances -> buckets, over all tiles -----------------------------------------------------------------------
+// One workgroup per (bucket, head): lists the bucket's distances in order, then adds their partial sums of every tile (64 bits, fixed order).
+// These workgroups are the last ones of the dk / dv launch, where they fill its tail; a launch of their own took 5 to 9 us (32 sequences
+// of 61 to 700 rows, 8 heads of 64, bf16, forward and backward: 184 -> 178 us).
+template <class T> __device__ __forceinline__ void at_dbias(const AtParams& P, int slots, int bucket, int head, unsigned char* smem) {
+  int* list = reinterpret_cast<int*>(smem);
+  int* kind = list + 2 * IRX_ATTN_MAX_FAR + 1;
+  double* red = reinterpret_cast<double*>(smem + (2 * (2 * IRX_ATTN_MAX_FAR + 1) * sizeof(int) + 15) / 16 * 16);
+  int* count = reinterpret_cast<int*>(red + 4);
+  const int heads = P.heads, far = P.far, buckets = P.buckets, W = 2 * far + 1;
+  const int32_t* map = P.map;
+  const float* part = P.part;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int d = threadIdx.x; d < W; d += 256) {
+    const int b = map[d];
+    kind[d] = b < 0 ? 0 : (b >= buckets ? buckets - 1 : b);
+  }
+  __syncthreads();
+  if (wave == 0) {
+    int n = 0;
+    for (int base = 0; base < W; base += 64) {
+      const int d = base + lane;
+      const bool in = d < W && kind[d < W ? d : 0] == bucket;
+      const unsigned long long hit = __ballot(in);
+      if (in) list[n + __popcll(hit & ((1ull << lane) - 1))] = d;
+      n += __popcll(hit);
+    }
+    if (lane == 0) *count = n;
+  }
+  __syncthreads();
+  const int c = *count;
+  double s = 0;
+  if (c) {
+    const long long n = (long long)slots * c;
+    const long long step = (1 << 30) / c * (long long)c;                 // whole tiles at a time, so that the divisions below are 32 bits
+    for (long long from = 0; from < n; from += step) {
+      const float* p0 = part + (size_t)(from / c) * heads * W;
+      const int m = (int)(n - from < step ? n - from : step);
+#pragma unroll 4
+      for (int i = threadIdx.x; i < m; i += 256) s += (double)p0[((size_t)(i / c) * heads + head) * W + list[i % c]];
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if (lane == 0) red[wave] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const float x = (float)(((red[0] + red[1]) + red[2]) + red[3]);
+    const size_t at = (size_t)bucket * heads + head;
+    if (P.table_f32 || T::ID == IRX_ATTN_F32) reinterpret_cast<float*>(P.dtable)[at] = x;
+    else if constexpr (T::ID == IRX_ATTN_BF16) reinterpret_cast<unsigned short*>(P.dtable)[at] = (unsigned short)irx_pk_bf16(x, 0.f);
+    else reinterpret_cast<_Float16*>(P.dtable)[at] = (_Float16)x;
+  }
+}
+
 // ---- dk, dv -----------------------------------------------------------------------------------------------------------------------
 template <class T, int D, bool BIAS>
-__global__ __launch_bounds__(256, (T::ESZ == 2 && D <= 64) ? 2 : 1) void k_attn_dkv(AtParams P, int total) {
+__global__ __launch_bounds__(256, (T::ESZ == 2 && D <= 64) ? 2 : 1) void k_attn_dkv(AtParams P, int total, int q_slots) {
   typedef AtTile<T, D> Tile;
   typedef typename T::F F;
   typedef typename T::S S;
   constexpr int STEPS = D / 16, BLOCKS = D / 32;
   // float16 keeps 10 bits below 2^-14: weights of long rows are that small, so they go through the product times 2^10
   constexpr float UP = T::ID == IRX_ATTN_F16 ? 1024.f : 1.f;
+  static_assert(4 * Tile::BYTES >= 16384, "the bias gradient's lists lie in the tiles' place");
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   float* srow = reinterpret_cast<float*>(smem + 4 * Tile::BYTES);        // [buffer][row maxima | 1 / row sums | D][64 queries]
   float* sb = srow + 6 * IRX_ATTN_BN;
 
-  const int per = gridDim.x >> 3;
+  const int per = (total + 7) >> 3;
+  if constexpr (BIAS) {
+    const int extra = (int)blockIdx.x - 8 * per;
+    if (extra >= 0) {
+      at_dbias<T>(P, q_slots, extra % P.buckets, extra / P.buckets, smem);
+      return;
+    }
+  }
   const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if (id >= total) return;
   const int slot = id % P.slots, rest = id / P.slots, kvh = rest % P.kv_heads, part = rest / P.kv_heads;
@@ -487,59 +550,6 @@ __global__ __launch_bounds__(256) void k_attn_dkv_join(AtParams P, size_t one) {
   at_st4<T>(to, s[0] * f, s[1] * f, s[2] * f, s[3] * f);
 }
 
-// ---- bias gradient: distances -> buckets, over all tiles -----------------------------------------------------------------------
-// One workgroup per (bucket, head): lists the bucket's distances in order, then adds their partial sums of every tile (64 bits, fixed order).
-template <class T>
-__global__ __launch_bounds__(256) void k_attn_dbias(const float* part, int slots, int heads, int far, const int32_t* map, int buckets,
-                                                    void* dtable, int table_f32) {
-  __shared__ int list[2 * IRX_ATTN_MAX_FAR + 1];
-  __shared__ int kind[2 * IRX_ATTN_MAX_FAR + 1];
-  __shared__ int count;
-  __shared__ double red[4];
-  const int bucket = blockIdx.x, head = blockIdx.y, W = 2 * far + 1;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int d = threadIdx.x; d < W; d += 256) {
-    const int b = map[d];
-    kind[d] = b < 0 ? 0 : (b >= buckets ? buckets - 1 : b);
-  }
-  __syncthreads();
-  if (wave == 0) {
-    int n = 0;
-    for (int base = 0; base < W; base += 64) {
-      const int d = base + lane;
-      const bool in = d < W && kind[d < W ? d : 0] == bucket;
-      const unsigned long long hit = __ballot(in);
-      if (in) list[n + __popcll(hit & ((1ull << lane) - 1))] = d;
-      n += __popcll(hit);
-    }
-    if (lane == 0) count = n;
-  }
-  __syncthreads();
-  const int c = count;
-  double s = 0;
-  if (c) {
-    const long long n = (long long)slots * c;
-    const long long step = (1 << 30) / c * (long long)c;                 // whole tiles at a time, so that the divisions below are 32 bits
-    for (long long from = 0; from < n; from += step) {
-      const float* p0 = part + (size_t)(from / c) * heads * W;
-      const int m = (int)(n - from < step ? n - from : step);
-#pragma unroll 4
-      for (int i = threadIdx.x; i < m; i += 256) s += (double)p0[((size_t)(i / c) * heads + head) * W + list[i % c]];
-    }
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  if (lane == 0) red[wave] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const float x = (float)(((red[0] + red[1]) + red[2]) + red[3]);
-    const size_t at = (size_t)bucket * heads + head;
-    if (table_f32 || T::ID == IRX_ATTN_F32) reinterpret_cast<float*>(dtable)[at] = x;
-    else if constexpr (T::ID == IRX_ATTN_BF16) reinterpret_cast<unsigned short*>(dtable)[at] = (unsigned short)irx_pk_bf16(x, 0.f);
-    else reinterpret_cast<_Float16*>(dtable)[at] = (_Float16)x;
-  }
-}
-
 // Parts of the query axis for dk / dv, by sizes alone: about four workgroups (128 keys of one key head each) per place on the chip, so
 // that the longest ones, the first keys of a long causal sequence, do not end alone. Two places per compute unit up to dimension 64 in 16
 // bits, else one (registers). Measured, us for the whole backward pass and forward: 12289 causal, 8 / 2 heads of 64: 1085 with 1024
@@ -563,12 +573,11 @@ template <class T, int D, bool BIAS> static int launch_bwd(AtParams P, void* dq,
     if (int rc = at_want_lds(reinterpret_cast<const void*>(&k_attn_dq<T, D, BIAS>), lds, "irx_attn_packed_bwd")) return rc;
     k_attn_dq<T, D, BIAS><<<(unsigned)((total + 7) / 8 * 8), 256, lds, st>>>(P, (int)total);
     IRX_CHECK_LAUNCH("irx_attn_packed_bwd(dq)");
-    if constexpr (BIAS) {
-      k_attn_dbias<T><<<dim3(P.buckets, P.heads), 256, 0, st>>>(P.part, P.slots, P.heads, P.far, P.map, P.buckets, dtable, P.table_f32);
-      IRX_CHECK_LAUNCH("irx_attn_packed_bwd(bias)");
-    }
   }
-  if (P.tk > 0) {
+  const int q_slots = P.slots;
+  if (P.tk > 0 || (BIAS && P.tq > 0)) {                                  // (no keys: the bias gradient is zero, and written)
+    const long long extra = BIAS && P.tq > 0 ? (long long)P.buckets * P.heads : 0;
+    P.dtable = dtable;
     P.slots = at_slots(P.tk, P.batch, IRX_ATTN_BM);
     P.dst = dk;
     P.dst2 = dv;
@@ -576,7 +585,7 @@ template <class T, int D, bool BIAS> static int launch_bwd(AtParams P, void* dq,
     const size_t lds = tiles + 6 * IRX_ATTN_BN * sizeof(float) + w;
     const long long total = (long long)P.slots * P.kv_heads * P.splits;
     if (int rc = at_want_lds(reinterpret_cast<const void*>(&k_attn_dkv<T, D, BIAS>), lds, "irx_attn_packed_bwd")) return rc;
-    k_attn_dkv<T, D, BIAS><<<(unsigned)((total + 7) / 8 * 8), 256, lds, st>>>(P, (int)total);
+    k_attn_dkv<T, D, BIAS><<<(unsigned)((total + 7) / 8 * 8 + extra), 256, lds, st>>>(P, (int)total, q_slots);
     IRX_CHECK_LAUNCH("irx_attn_packed_bwd(dkv)");
     if (P.splits > 1) {
       const size_t one = (size_t)P.tk * P.kv_heads * D;

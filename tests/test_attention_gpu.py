@@ -113,6 +113,19 @@ def test_position_bias_that_forbids_buckets():
         assert float(t.abs().max()) == 0.0, n
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_bias_gradient_without_keys_and_of_many_buckets(kind, backend):
+    table = torch.randn(700, 3, generator=torch.Generator().manual_seed(13))
+    buckets = torch.arange(700, dtype=torch.int32)[:2 * 340 + 1]              # a bucket per distance, some that none has
+    compare([300, 64], [300, 20], 3, 3, 32, kind, False, table=table, buckets=buckets, seed=14)
+    junk = [torch.full((700, 3), math.nan, device=DEV) for _ in range(8)]      # what lies where the result will
+    del junk
+    q, k, v, do = make([70, 5], [0, 0], 3, 3, 64, TYPES[kind], 15)
+    got = run(q, k, v, offsets([70, 5]), offsets([0, 0]), do, False, None, table, buckets)
+    for n, t in got.items():
+        assert not t.numel() or float(t.abs().max()) == 0.0, n
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_lowest_bias_beyond_the_clipped_distance(kind, dim):
