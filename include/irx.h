@@ -649,8 +649,8 @@ int irx_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* 
  * out, dq [tq][heads][dim], dk, dv [tk][kv_heads][dim] contiguous; stats float32 [heads][tq][2] is what the backward needs of the
  * forward (NULL: not written); rest, like out and in 16 bits only: what out's rounding left over, which makes the gradients more exact
  * (NULL in the forward: not kept, in the backward: none); dtable like table. Offsets are read on the device only: no length has to be known on the host.
- * Deterministic. irx_attn_packed_bwd_workspace_bytes: far = -1 without a bias table. */
-size_t irx_attn_packed_fwd_workspace_bytes(int tq, int tk, int batch, int heads, int kv_heads, int dim, int dtype, int bias);
+ * Deterministic. irx_attn_packed_fwd_workspace_bytes: mask = 1 with a bias table, + 2 when causal; _bwd_: far = -1 without a bias table. */
+size_t irx_attn_packed_fwd_workspace_bytes(int tq, int tk, int batch, int heads, int kv_heads, int dim, int dtype, int mask);
 int irx_attn_packed_fwd(const void* q, long long q_row, long long q_head, const void* k, long long k_row, long long k_head,
                         const void* v, long long v_row, long long v_head, const int32_t* cu_q, const int32_t* cu_k, int batch, int tq,
                         int tk, int heads, int kv_heads, int dim, int dtype, float scale, int causal, const void* table,

@@ -95,7 +95,8 @@ def _forward(q, k, v, table, cu_q, cu_k, causal, scale, buckets, want_stats):
     out = torch.empty((tq, heads, dim), dtype=q.dtype, device=q.device)
     stats = torch.empty((heads, tq, 2), dtype=torch.float32, device=q.device) if want_stats else None
     rest = torch.empty_like(out) if want_stats and q.dtype != torch.float32 else None      # what the output's rounding leaves over
-    n = int(_lib.load().irx_attn_packed_fwd_workspace_bytes(tq, tk, batch, heads, kv_heads, dim, _TYPES[q.dtype], table is not None))
+    n = int(_lib.load().irx_attn_packed_fwd_workspace_bytes(tq, tk, batch, heads, kv_heads, dim, _TYPES[q.dtype],
+                                                              (table is not None) + (2 if causal else 0)))
     ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     tb, tb_f32, mp, nb, far = _table_args(table, buckets)
     _lib.call("irx_attn_packed_fwd", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),

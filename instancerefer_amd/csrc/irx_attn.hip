@@ -339,15 +339,17 @@ __global__ __launch_bounds__((64 * few_waves<T, D>())) void k_attn_few(AtParams 
   }
 }
 
-// Joins the parts of a row: o = sum_p w_p o_p / sum_p w_p, w_p = l_p 2^(m_p - max m). One workgroup per row (head, query): groups of
-// D / 4 threads take every G-th part, their sums are joined in the groups' order: always the same result.
-template <class T, int D>
+// Joins the parts of a row: o = sum_p w_p o_p / sum_p w_p, w_p = l_p 2^(m_p - max m), by groups of D / 4 threads. Many rows (MANY): a group
+// per row, parts in order. Few: a workgroup per row, group g takes every G-th part, the groups' sums are joined in their order. Always the
+// same result. 98 312 rows of 64 in two parts: 15 us by groups, 112 by workgroups (idle groups); 256 rows of 128 in 64 parts: 9 and 4.
+template <class T, int D, bool MANY>
 __global__ __launch_bounds__(256) void k_attn_join(AtParams P) {
   constexpr int PER = D / 4, G = 256 / PER;
   __shared__ at_f32x4 so[G][PER];
   __shared__ float sl[G];
-  const size_t row = blockIdx.x, rows = (size_t)P.heads * P.tq;          // head * tq + q
   const int c = threadIdx.x % PER, g = threadIdx.x / PER, d = 4 * c;
+  const size_t row = MANY ? (size_t)blockIdx.x * G + g : blockIdx.x, rows = (size_t)P.heads * P.tq;          // head * tq + q
+  if (MANY && row >= rows) return;
   float M = -INFINITY;
 #pragma unroll 4
   for (int p = 0; p < P.splits; ++p) M = fmaxf(M, P.sst[2 * (p * rows + row)]);
@@ -355,7 +357,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AtParams P) {
   float L = 0.f;
   at_f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int p = g; p < P.splits; p += G) {
+  for (int p = MANY ? 0 : g; p < P.splits; p += MANY ? 1 : G) {
     const float l = P.sst[2 * (p * rows + row) + 1];
     const at_f32x4 x = *reinterpret_cast<const at_f32x4*>(P.so + (p * rows + row) * D + d);
     const float w = l == 0.f ? 0.f : l * at_exp2(P.sst[2 * (p * rows + row)] - Ms);
@@ -363,15 +365,17 @@ __global__ __launch_bounds__(256) void k_attn_join(AtParams P) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(w, x[i], o[i]);
   }
-  so[g][c] = o;
-  if (c == 0) sl[g] = L;
-  __syncthreads();
-  if (g) return;
-  L = sl[0];
+  if constexpr (!MANY) {
+    so[g][c] = o;
+    if (c == 0) sl[g] = L;
+    __syncthreads();
+    if (g) return;
+    L = sl[0];
 #pragma unroll
-  for (int i = 1; i < G; ++i) {
-    L += sl[i];
-    o += so[i][c];
+    for (int i = 1; i < G; ++i) {
+      L += sl[i];
+      o += so[i][c];
+    }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   const size_t head = row / P.tq, q = row % P.tq;
@@ -384,8 +388,12 @@ __global__ __launch_bounds__(256) void k_attn_join(AtParams P) {
   }
 }
 
+// (512 workgroups of rows: two per compute unit, from there on the parts are read at memory speed)
 template <class T, int D> static int launch_join(const AtParams& P, hipStream_t st) {
-  k_attn_join<T, D><<<(unsigned)((size_t)P.heads * P.tq), 256, 0, st>>>(P);
+  constexpr int G = 256 / (D / 4);
+  const size_t rows = (size_t)P.heads * P.tq;
+  if (rows >= 512 * G) k_attn_join<T, D, true><<<(unsigned)((rows + G - 1) / G), 256, 0, st>>>(P);
+  else k_attn_join<T, D, false><<<(unsigned)rows, 256, 0, st>>>(P);
   IRX_CHECK_LAUNCH("irx_attn_packed_fwd(join)");
   return IRX_OK;
 }
@@ -447,10 +455,14 @@ int at_check(const char* who, const AtParams& P, int dim, int dtype, int elem) {
 }
 
 // How the forward is launched, by sizes alone. Few: the average sequence's queries, times the heads that share a key head, fit one tile
-// of 32 rows, and there are many keys (16 single tokens over 500 to 8100 keys, 16 / 4 heads of 128: 35 us with the join, without it 83; about 256 workgroups: 512 41, 1024 51). Else parts of
-// the key axis only where the whole launch is far below one workgroup per compute unit. tokens: queries of a few-row tile, 0: no.
+// of 32 rows, and there are many keys (16 single tokens over 500 to 8100 keys, 16 / 4 heads of 128: 35 us with the join, without it 83;
+// about 256 workgroups: 512 41, 1024 51). Else parts of the key axis only where the whole launch is below a round of two workgroups per
+// compute unit (4096 causal rows, 8 heads of 64, bf16: 67 us whole, 54 in three parts; 2048 rows, 16 heads of 128, full: 67 whole, 57 in two, 66 in
+// three; 16000 causal, 4 heads of 128: 389 whole, 285 in two) or, causal, not far above it (12289 rows, 8 heads of 64,
+// fp16: 245 and 222; 6000 rows, 12 heads of 64: 136 and 104; but 6000 rows, 16 heads of 128: 168 and 186, so the rule weighs the keys, which
+// make the join cheap, against how full the second round is). tokens: queries of a few-row tile, 0: no.
 struct FwdPlan { int tokens, splits; };
-static FwdPlan fwd_plan(long long tq, long long tk, int batch, int heads, int kv_heads, int dim, int elem, bool bias) {
+static FwdPlan fwd_plan(long long tq, long long tk, int batch, int heads, int kv_heads, int dim, int elem, bool bias, bool causal) {
   if (batch <= 0 || tk <= 0 || tq <= 0) return {0, 1};
   const long long keys = tk / batch, busy = batch < tq ? batch : tq;
   const int group = heads / kv_heads;
@@ -463,15 +475,20 @@ static FwdPlan fwd_plan(long long tq, long long tk, int batch, int heads, int kv
     return {tokens, (int)s * waves};
   }
   const long long wgs = (tq / IRX_ATTN_BM + busy) * heads;
-  if (wgs >= 512 || keys < 1024) return {0, 1};
-  long long s = 1024 / wgs;
+  if (keys < 1024) return {0, 1};
+  if (wgs >= 512) {
+    // one round and a half of workgroups: under a causal mask the longest tiles end last, two parts even it out for a join of 8 bytes per value
+    const bool even = causal && wgs < 1024 && keys * (1024 - wgs) * (elem == 4 ? 4 : 1) >= 1 << 21;
+    return {0, even ? 2 : 1};
+  }
+  long long s = wgs > 266 ? 2 : 800 / wgs;
   if (s > keys / 256) s = keys / 256;
-  return {0, s < 1 ? 1 : s > 32 ? 32 : (int)s};
+  return {0, s > 32 ? 32 : (int)s};
 }
 
-extern "C" size_t irx_attn_packed_fwd_workspace_bytes(int tq, int tk, int batch, int heads, int kv_heads, int dim, int dtype, int bias) {
+extern "C" size_t irx_attn_packed_fwd_workspace_bytes(int tq, int tk, int batch, int heads, int kv_heads, int dim, int dtype, int mask) {
   if (tq <= 0 || tk < 0 || batch < 0 || heads <= 0 || kv_heads <= 0 || dim <= 0) return 0;
-  const int s = fwd_plan(tq, tk, batch, heads, kv_heads, dim, dtype == IRX_ATTN_F32 ? 4 : 2, bias != 0).splits;
+  const int s = fwd_plan(tq, tk, batch, heads, kv_heads, dim, dtype == IRX_ATTN_F32 ? 4 : 2, mask & 1, mask & 2).splits;
   return s <= 1 ? 0 : (size_t)s * heads * tq * (dim + 2) * sizeof(float);
 }
 
@@ -492,10 +509,10 @@ extern "C" int irx_attn_packed_fwd(const void* q, long long q_row, long long q_h
   if (tq == 0) return IRX_OK;
   IRX_REQUIRE(out && (((uintptr_t)out | (uintptr_t)rest) & 15) == 0, "irx_attn_packed_fwd: out must be given and start on 16 bytes");
   P.slots = at_slots(tq, batch, IRX_ATTN_BM);
-  const FwdPlan plan = fwd_plan(tq, tk, batch, heads, kv_heads, dim, dtype == IRX_ATTN_F32 ? 4 : 2, table != nullptr);
+  const FwdPlan plan = fwd_plan(tq, tk, batch, heads, kv_heads, dim, dtype == IRX_ATTN_F32 ? 4 : 2, table != nullptr, causal != 0);
   P.splits = plan.splits;
   if (P.splits > 1) {
-    const size_t need = irx_attn_packed_fwd_workspace_bytes(tq, tk, batch, heads, kv_heads, dim, dtype, table != nullptr);
+    const size_t need = irx_attn_packed_fwd_workspace_bytes(tq, tk, batch, heads, kv_heads, dim, dtype, (table != nullptr) + 2 * (causal != 0));
     if (!workspace || workspace_bytes < need) {
       irx_set_error("irx_attn_packed_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
       return IRX_ERR_WORKSPACE;

@@ -104,7 +104,7 @@ Tensor attn_forward(const Attn& a, Tensor* stats, Tensor* rest, void* stream) {
   Tensor out = at::empty({tq, heads, dim}, q.options());
   if (stats) *stats = at::empty({heads, tq, 2}, q.options().dtype(at::kFloat));
   if (rest && q.scalar_type() != at::kFloat) *rest = at::empty_like(out);
-  const size_t n = g_text.attn_fwd_ws(tq, tk, a.batch(), heads, kv, dim, type_of(q), a.table.defined());
+  const size_t n = g_text.attn_fwd_ws(tq, tk, a.batch(), heads, kv, dim, type_of(q), a.table.defined() + 2 * a.causal);
   const Tensor ws = n ? bytes(n, q) : Tensor();
   const bool b = a.table.defined();
   check(g_text.attn_fwd(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), a.v.data_ptr(), a.v.stride(0), a.v.stride(1),

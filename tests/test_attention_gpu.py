@@ -113,6 +113,17 @@ def test_position_bias_that_forbids_buckets():
         assert float(t.abs().max()) == 0.0, n
 
 
+@pytest.mark.parametrize("kind,heads,kv,dim,causal", [("bf16", 16, 4, 32, False), ("f16", 9, 3, 64, True), ("f32", 4, 4, 128, True), ("f32", 60, 20, 32, True)])
+def test_key_axis_in_parts_with_many_rows(kind, heads, kv, dim, causal):
+    """parts of the key axis joined row by row, several rows to a workgroup; the last case: two parts although the launch fills the chip"""
+    from instancerefer_amd import _lib
+    rows = 1101
+    code, mask = {"f32": 0, "bf16": 1, "f16": 2}[kind], 2 * causal
+    assert _lib.load().irx_attn_packed_fwd_workspace_bytes(rows, rows, 1, heads, kv, dim, code, mask) > 0
+    assert rows * heads * (dim // 4) >= 512 * 256
+    compare([rows], [rows], heads, kv, dim, kind, causal, seed=16)
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16"])
 def test_bias_gradient_without_keys_and_of_many_buckets(kind, backend):
     table = torch.randn(700, 3, generator=torch.Generator().manual_seed(13))
