@@ -54,7 +54,7 @@ struct AtParams {
   float* part;                               // backward: bias gradient by distance, [slots][heads][2 far + 1]
   void* dtable;                              // ... and by bucket, the result
   int slots;
-  int splits; float* so; float* sst;         // forward over a long axis in parts: partial outputs and (max, sum)
+  int splits; float* so; float* sst;         // a long axis in parts: partial results and, forward, (max, sum)
 };
 
 // ---- which rows a workgroup owns ------------------------------------------------------------------------------------------
@@ -96,6 +96,19 @@ __device__ __forceinline__ AtSpan at_span(const int32_t* cu, int batch, int tota
 }
 
 static inline int at_slots(int total, int batch, int bm) { return total / bm + batch + 2; }
+
+// Parts of the key axis for a kernel that owns queries, `wgs` workgroups of 128 rows over about `keys` keys each. Measured: irx_attn.hip's
+// and irx_attn_bwd.hip's launches.
+static inline int at_key_parts(long long wgs, long long keys, int elem, bool causal) {
+  if (keys < 1024) return 1;
+  if (wgs >= 512) {
+    // one round and a half of workgroups: under a causal mask the longest tiles end last, two parts even it out for a join of 8 bytes per value
+    return causal && wgs < 1024 && keys * (1024 - wgs) * (elem == 4 ? 4 : 1) >= 1 << 21 ? 2 : 1;
+  }
+  long long s = wgs > 266 ? 2 : 800 / wgs;
+  if (s > keys / 256) s = keys / 256;
+  return s > 32 ? 32 : (int)s;
+}
 
 // ---- fragments ------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ at_f32x16 at_mma(at_bf16x8 a, at_bf16x8 b, at_f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }

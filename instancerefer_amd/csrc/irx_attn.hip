@@ -475,15 +475,7 @@ static FwdPlan fwd_plan(long long tq, long long tk, int batch, int heads, int kv
     return {tokens, (int)s * waves};
   }
   const long long wgs = (tq / IRX_ATTN_BM + busy) * heads;
-  if (keys < 1024) return {0, 1};
-  if (wgs >= 512) {
-    // one round and a half of workgroups: under a causal mask the longest tiles end last, two parts even it out for a join of 8 bytes per value
-    const bool even = causal && wgs < 1024 && keys * (1024 - wgs) * (elem == 4 ? 4 : 1) >= 1 << 21;
-    return {0, even ? 2 : 1};
-  }
-  long long s = wgs > 266 ? 2 : 800 / wgs;
-  if (s > keys / 256) s = keys / 256;
-  return {0, s > 32 ? 32 : (int)s};
+  return {0, at_key_parts(wgs, keys, elem, causal)};
 }
 
 extern "C" size_t irx_attn_packed_fwd_workspace_bytes(int tq, int tk, int batch, int heads, int kv_heads, int dim, int dtype, int mask) {

@@ -64,13 +64,13 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
   const int per = gridDim.x >> 3;
   const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if (id >= total) return;
-  const int slot = P.slots - 1 - id % P.slots, head = id / P.slots;
+  const int slot = P.slots - 1 - id % P.slots, hs = id / P.slots, head = hs % P.heads, part = hs / P.heads;
 
   int first;
   const AtSpan sp = at_span(P.cu_q, P.batch, P.tq, IRX_ATTN_BM, slot, &first);
   if (sp.begin >= sp.end) {
     if constexpr (BIAS)
-      for (int d = threadIdx.x; d < W; d += 256) P.part[((size_t)slot * P.heads + head) * W + d] = 0.f;
+      for (int d = threadIdx.x; d < W; d += 256) P.part[(((size_t)part * P.slots + slot) * P.heads + head) * W + d] = 0.f;
     return;
   }
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -89,7 +89,12 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
   const int wave_full = row0 + 32 > sp.end ? 0 : (P.causal ? min(lk, i0 + 1 + off) : lk);
   const int wave_any = row0 >= sp.end ? 0 : (P.causal ? min(lk, min(i0 + 32, sp.end - first) + off) : lk);
   const int block_any = P.causal ? min(lk, min(sp.begin + IRX_ATTN_BM, sp.end) - first + off) : lk;
-  const int t1 = (max(block_any, 0) + IRX_ATTN_BN - 1) / IRX_ATTN_BN;
+  int t0 = 0, t1 = (max(block_any, 0) + IRX_ATTN_BN - 1) / IRX_ATTN_BN;
+  if (P.splits > 1) {
+    const int n = t1;
+    t0 = (int)((long long)n * part / P.splits);
+    t1 = (int)((long long)n * (part + 1) / P.splits);
+  }
   const int kvh = head / (P.heads / P.kv_heads);
   const S* kp = reinterpret_cast<const S*>(P.k.p) + kb * P.k.st + kvh * P.k.sh;
   const S* vp = reinterpret_cast<const S*>(P.v.p) + kb * P.v.st + kvh * P.v.sh;
@@ -116,7 +121,7 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
       const float* st = P.stats + ((size_t)head * P.tq + q) * 2;
       m = st[0];
       inv = st[1];
-      if (half == 0) P.delta[(size_t)head * P.tq + q] = delta;
+      if (half == 0 && part == 0) P.delta[(size_t)head * P.tq + q] = delta;
     }
   }
   if constexpr (BIAS) {
@@ -138,18 +143,18 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
   Tile::dma_offsets(ko, ks);
   Tile::dma_offsets(vo, vs);
   auto fetch = [&](int t) __attribute__((always_inline)) {
-    const unsigned to = lds0 + (t % BUFS) * 2 * Tile::BYTES;
+    const unsigned to = lds0 + ((t - t0) % BUFS) * 2 * Tile::BYTES;
     const int k0 = t * IRX_ATTN_BN;
     Tile::dma(to, kp + k0 * P.k.st, ks, lk - k0, ko);
     Tile::dma(to + Tile::BYTES, vp + k0 * P.v.st, vs, lk - k0, vo);
   };
-  if (t1 > 0) fetch(0);
-  for (int t = 0; t < t1; ++t) {
+  if (t0 < t1) fetch(t0);
+  for (int t = t0; t < t1; ++t) {
     const int k0 = t * IRX_ATTN_BN;
     at_landed();
     __syncthreads();
     if (BUFS == 2 && t + 1 < t1) fetch(t + 1);
-    const unsigned char* lk_ = smem + (t % BUFS) * 2 * Tile::BYTES;
+    const unsigned char* lk_ = smem + ((t - t0) % BUFS) * 2 * Tile::BYTES;
     const unsigned char* lv_ = lk_ + Tile::BYTES;
 #pragma unroll
     for (int kb2 = 0; kb2 < 2; ++kb2) {
@@ -245,16 +250,36 @@ __global__ __launch_bounds__(256, T::ESZ == 2 ? 2 : 1) void k_attn_dq(AtParams P
       float s = 0.f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) s += sd[w * W + d];
-      P.part[((size_t)slot * P.heads + head) * W + d] = s;
+      P.part[(((size_t)part * P.slots + slot) * P.heads + head) * W + d] = s;
     }
   }
   if (!mine) return;
-  S* o = reinterpret_cast<S*>(P.dst) + ((size_t)q * P.heads + head) * D + 4 * half;
+  const size_t at = ((size_t)q * P.heads + head) * D + 4 * half;
+  if (P.splits > 1) {
+    float* o = P.so + (size_t)part * P.tq * P.heads * D + at;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        at_st4<AtF32>(o + 32 * b + 8 * g, acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]);
+    return;
+  }
+  S* o = reinterpret_cast<S*>(P.dst) + at;
 #pragma unroll
   for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
     for (int g = 0; g < 4; ++g)
       at_st4<T>(o + 32 * b + 8 * g, acc[b][4 * g] * P.scale, acc[b][4 * g + 1] * P.scale, acc[b][4 * g + 2] * P.scale, acc[b][4 * g + 3] * P.scale);
+}
+
+// adds the parts of dq in their order and rounds
+template <class T>
+__global__ __launch_bounds__(256) void k_attn_dq_join(AtParams P, size_t n) {
+  const size_t at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= n) return;
+  at_f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < P.splits; ++p) s += *reinterpret_cast<const at_f32x4*>(P.so + p * n + at);
+  at_st4<T>(reinterpret_cast<typename T::S*>(P.dst) + at, s[0] * P.scale, s[1] * P.scale, s[2] * P.scale, s[3] * P.scale);
 }
 
 // ---- bias gradient: distances -> buckets, over all tiles -----------------------------------------------------------------------
@@ -563,18 +588,32 @@ static int dkv_splits(long long tq, long long tk, int batch, int heads, int kv_h
   return s < 1 ? 1 : s > 8 ? 8 : (int)s;
 }
 
+// Parts of the key axis for dq, by sizes alone, as for the forward. Measured, backward pass, us without and with:
+// 4096 causal rows, 8 heads of 64, bf16: 163, 144; 6000 rows, 12 heads: 340, 290; 3000 rows, 4 heads of 64, float32: 445, 242; 12289 rows,
+// 8 heads, fp16: 697, 692; 1024 rows, 16 heads: 66, 69.
+static int dq_splits(long long tq, long long tk, int batch, int heads, int elem, bool causal) {
+  if (batch <= 0 || tk <= 0 || tq <= 0) return 1;
+  return at_key_parts((tq / IRX_ATTN_BM + (batch < tq ? batch : tq)) * heads, tk / batch, elem, causal);
+}
+
 template <class T, int D, bool BIAS> static int launch_bwd(AtParams P, void* dq, void* dk, void* dv, void* dtable, hipStream_t st) {
   const size_t tiles = 4 * AtTile<T, D>::BYTES, w = BIAS ? sizeof(float) * (2 * P.far + 1) : 0;
   if (P.tq > 0) {
     P.slots = at_slots(P.tq, P.batch, IRX_ATTN_BM);
     P.dst = dq;
     const size_t lds = (BIAS && T::ESZ == 4 && D == 128 ? tiles / 2 : tiles) + 5 * w;
-    const long long total = (long long)P.slots * P.heads;
+    P.splits = dq_splits(P.tq, P.tk, P.batch, P.heads, T::ESZ, P.causal);
+    const long long total = (long long)P.slots * P.heads * P.splits;
     if (int rc = at_want_lds(reinterpret_cast<const void*>(&k_attn_dq<T, D, BIAS>), lds, "irx_attn_packed_bwd")) return rc;
     k_attn_dq<T, D, BIAS><<<(unsigned)((total + 7) / 8 * 8), 256, lds, st>>>(P, (int)total);
     IRX_CHECK_LAUNCH("irx_attn_packed_bwd(dq)");
+    if (P.splits > 1) {
+      const size_t n = (size_t)P.tq * P.heads * D;
+      k_attn_dq_join<T><<<(unsigned)((n / 4 + 255) / 256), 256, 0, st>>>(P, n);
+      IRX_CHECK_LAUNCH("irx_attn_packed_bwd(dq join)");
+    }
   }
-  const int q_slots = P.slots;
+  const int q_slots = P.slots * P.splits;                                // tiles and parts that hold bias sums
   if (P.tk > 0 || (BIAS && P.tq > 0)) {                                  // (no keys: the bias gradient is zero, and written)
     const long long extra = BIAS && P.tq > 0 ? (long long)P.buckets * P.heads : 0;
     P.dtable = dtable;
@@ -602,15 +641,16 @@ template <class T> static int launch_bwd_d(const AtParams& P, int dim, void* dq,
   return dim == 32 ? launch_bwd_b<T, 32>(P, dq, dk, dv, dt, st) : dim == 64 ? launch_bwd_b<T, 64>(P, dq, dk, dv, dt, st) : launch_bwd_b<T, 128>(P, dq, dk, dv, dt, st);
 }
 
-// D, then (aligned) the parts of dk and dv, then the bias gradient by distance
+// D, then (aligned) the parts of dq or, later, of dk and dv, then the bias gradient by distance (counted as if causal: the most there is)
 static size_t bwd_delta(int tq, int heads) { return ((size_t)heads * tq + 3) / 4 * 4; }
 static size_t bwd_parts(int tq, int tk, int batch, int heads, int kv_heads, int dim, int elem) {
-  const int s = dkv_splits(tq, tk, batch, heads, kv_heads, dim, elem);
-  return s > 1 ? (size_t)s * 2 * tk * kv_heads * dim : 0;
+  const int s = dkv_splits(tq, tk, batch, heads, kv_heads, dim, elem), r = dq_splits(tq, tk, batch, heads, elem, true);
+  const size_t kv = s > 1 ? (size_t)s * 2 * tk * kv_heads * dim : 0, q = r > 1 ? (size_t)r * tq * heads * dim : 0;
+  return kv > q ? kv : q;
 }
 extern "C" size_t irx_attn_packed_bwd_workspace_bytes(int tq, int tk, int batch, int heads, int kv_heads, int dim, int dtype, int far) {
   if (tq <= 0 || tk < 0 || batch < 0 || heads <= 0 || kv_heads <= 0 || dim <= 0) return 0;
-  const size_t part = far < 0 ? 0 : (size_t)at_slots(tq, batch, IRX_ATTN_BM) * heads * (2 * (size_t)far + 1);
+  const size_t part = far < 0 ? 0 : (size_t)at_slots(tq, batch, IRX_ATTN_BM) * dq_splits(tq, tk, batch, heads, dtype == IRX_ATTN_F32 ? 4 : 2, true) * heads * (2 * (size_t)far + 1);
   return (bwd_delta(tq, heads) + bwd_parts(tq, tk, batch, heads, kv_heads, dim, dtype == IRX_ATTN_F32 ? 4 : 2) + part) * sizeof(float);
 }
 

@@ -124,6 +124,13 @@ def test_key_axis_in_parts_with_many_rows(kind, heads, kv, dim, causal):
     compare([rows], [rows], heads, kv, dim, kind, causal, seed=16)
 
 
+@pytest.mark.parametrize("kind,dim,causal", [("bf16", 64, True), ("f32", 128, False), ("f16", 32, True)])
+def test_key_axis_in_parts_with_a_bias(kind, dim, causal, backend):
+    from instancerefer_amd.attention import relative_buckets
+    table = torch.randn(12, 4, generator=torch.Generator().manual_seed(17))
+    compare([1300, 40, 1100], [1300, 900, 1100], 4, 2, dim, kind, causal, table=table, buckets=relative_buckets(12, 60, not causal), seed=18)
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16"])
 def test_bias_gradient_without_keys_and_of_many_buckets(kind, backend):
     table = torch.randn(700, 3, generator=torch.Generator().manual_seed(13))
