@@ -7,8 +7,8 @@
 // are computed in both: 7 products in place of 5. Both use the transposed layouts of irx_attn.h: P and dS are operands as they come.
 // P and dS are rounded to the operand type for the second products; row statistics, D, dS itself and all sums are 32 bits. D is formed
 // from the stored output and what its rounding left over, where the forward kept that.
-// Measured: 12289 causal rows, 8 / 2 heads of 64, float16: dq 305 us (760 TFLOP/s of its three products), dk / dv 378 us (820 of its
-// four) and 16 us for the join of its parts. Six causal sequences of 130 to 2719 rows, 16 / 4 heads of 128, bf16: 150 us (660), 276 us
+// Measured: 12289 causal rows, 8 / 2 heads of 64, float16: dq 290 us in two parts (800 TFLOP/s of its three products) and 10 for their
+// join, dk / dv 382 us (810 of its four) and 16. Six causal sequences of 130 to 2719 rows, 16 / 4 heads of 128, bf16: 160 us (620), 277 us
 // (480: its accumulators leave one wave per SIMD; with values in LDS and two waves 314 us, the registers spill). Bound there as the
 // forward is: matrix and vector instructions take turns.
 #include "irx_attn.h"

@@ -1,7 +1,7 @@
 // text_nodes.cpp — C++ autograd nodes of the text encoder's operators over the C-ABI (include/irx.h): packed attention and the
 // root-mean-square norm with the residual's addition. The same calls in the same order as the Python nodes (attention.py, dense.py); what
-// they save is the interpreter: a small norm's forward + backward is 150 us of host time through torch.autograd.Function, 100 here, of which
-// 65 are the autograd engine's call (51 for torch's own layer norm).
+// they save is the interpreter: a small norm's forward + backward is 150 us of host time through torch.autograd.Function, 76 here, of which
+// 51 are the autograd engine's call (50 for torch's own layer norm).
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
