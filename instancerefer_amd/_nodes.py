@@ -69,24 +69,32 @@ def _load_locked():
     return mod
 
 
-def refuse_foreign_leaves(who, leaves):
-    """Called under a graph capture, before a node on `leaves` is made or run backward: raises when one of them still belongs to an eager
-    graph of another stream. Its backward would make that stream wait inside the capture, which ends the process when the capture ends."""
+def _text_module(who):
     mod = load()
     if mod is None:
         raise RuntimeError("%s: gradients can be captured into a graph only with csrc/_irx_nodes.so (python -m instancerefer_amd._build)" % who)
-    i = mod.foreign_leaf(list(leaves))
+    return mod
+
+
+def _refuse(who, i):
     if i >= 0:
         raise RuntimeError("%s: a backward pass cannot be captured while an eager graph of the same leaves lives (input %d was used on "
                            "another stream): drop that graph's outputs first, or run the warm-up on the capture's stream" % (who, i))
+
+
+def refuse_foreign_leaves(who, leaves):
+    """Called under a graph capture, before a node on `leaves` is made: raises when one of them still belongs to an eager graph of
+    another stream. Its backward would make that stream wait inside the capture, which ends the process when the capture ends."""
+    _refuse(who, _text_module(who).foreign_leaf(list(leaves)))
+
+
+def refuse_foreign_behind(who):
+    """refuse_foreign_leaves inside a node's backward, for the leaves that this pass will feed: those right behind the node and those
+    behind copies and views that an operator made of them."""
+    _refuse(who, _text_module(who).foreign_behind())
 
 
 def refuse_capture_of_copies(who, tensors):
     """refuse_foreign_leaves for an operator that copies its inputs before its node sees them"""
     if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing() and any(t is not None and t.requires_grad for t in tensors):
         refuse_foreign_leaves(who, tensors)
-
-
-def leaves_of(ctx):
-    """the leaf tensors right behind a Python autograd.Function's node"""
-    return [n.variable for n, _ in ctx.next_functions if n is not None and hasattr(n, "variable")]

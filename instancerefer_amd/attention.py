@@ -123,7 +123,7 @@ class AttentionPackedFn(torch.autograd.Function):
         q, k, v, table, cu_q, cu_k, buckets, out, stats, rest = ctx.saved_tensors
         causal, scale = ctx.cfg
         if torch.cuda.is_current_stream_capturing():
-            _nodes.refuse_foreign_leaves("attention_packed", _nodes.leaves_of(ctx))
+            _nodes.refuse_foreign_behind("attention_packed")
         tq, heads, dim = q.shape
         tk, kv_heads, _ = k.shape
         batch = cu_q.shape[0] - 1

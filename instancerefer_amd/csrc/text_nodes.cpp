@@ -3,12 +3,15 @@
 // they save is the interpreter: a small norm's forward + backward is 150 us of host time through torch.autograd.Function, 76 here, of which
 // 51 are the autograd engine's call (50 for torch's own layer norm).
 #include <c10/core/impl/VirtualGuardImpl.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/extension.h>
 
 #include "torch_nodes.h"
 
 #include <unordered_map>
+#include <unordered_set>
 
 namespace irxn {
 
@@ -18,19 +21,64 @@ using torch::autograd::variable_list;
 typedef c10::optional<Tensor> OptTensor;
 typedef long long ll;
 
-// The first of `leaves` whose gradient accumulator lives on another stream than the current one of its device, or -1. The autograd engine
-// makes an accumulator's stream wait for the backward that feeds it, and the accumulator keeps the stream of the first graph that used the
-// leaf for as long as any such graph lives. Inside a capture that wait would draw a stream that is not being captured into it: the runtime
-// ends the process when the capture ends.
+// The autograd engine makes an accumulator's stream wait for the backward that feeds it, and the accumulator keeps the stream of the first
+// graph that used the leaf for as long as any such graph lives. Inside a capture that wait would draw a stream that is not being captured
+// into it: the runtime ends the process when the capture ends.
+static bool is_foreign(torch::autograd::Node& accumulator, const Tensor& leaf) {
+  const auto s = accumulator.stream();
+  return s.has_value() && *s != c10::impl::VirtualGuardImpl(leaf.device().type()).getStream(leaf.device());
+}
+
+// The first of `leaves` whose gradient accumulator lives on another stream than the current one of its device, or -1.
 static int64_t foreign_leaf(const std::vector<OptTensor>& leaves) {
   for (size_t i = 0; i < leaves.size(); ++i) {
     const auto& t = leaves[i];
     if (!t.has_value() || !t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
     const auto acc = torch::autograd::impl::try_get_grad_accumulator(*t);
-    if (!acc) continue;
-    const auto s = acc->stream();
-    if (s.has_value() && *s != c10::impl::VirtualGuardImpl(t->device().type()).getStream(t->device())) return (int64_t)i;
+    if (acc && is_foreign(*acc, *t)) return (int64_t)i;
   }
+  return -1;
+}
+
+// Inside a node's backward: the accumulators that this pass will feed right behind it, or behind copies and views of a leaf (an operator
+// pads and copies what its kernels cannot read in place), each with the number of the input that leads to it.
+static std::vector<std::pair<int64_t, torch::autograd::AccumulateGrad*>> accumulators_behind() {
+  using torch::autograd::Node;
+  static const std::unordered_set<std::string> kept = {
+      "CloneBackward0", "ConstantPadNdBackward0", "ToCopyBackward0", "AliasBackward0", "ViewBackward0", "UnsafeViewBackward0", "ReshapeAliasBackward0",
+      "AsStridedBackward0", "TransposeBackward0", "TBackward0", "PermuteBackward0", "UnsqueezeBackward0", "SqueezeBackward0", "SqueezeBackward1",
+      "SqueezeBackward2", "ExpandBackward0", "SliceBackward0", "SelectBackward0", "SplitBackward0", "SplitWithSizesBackward0", "UnbindBackward0"};
+  std::vector<std::pair<int64_t, torch::autograd::AccumulateGrad*>> out;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return out;
+  const auto* exec = torch::autograd::get_current_graph_task_exec_info();     // empty: everything runs
+  auto runs = [&](Node* n) {
+    if (!exec || exec->empty()) return true;
+    const auto it = exec->find(n);
+    return it != exec->end() && it->second.should_execute();
+  };
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    Node* n = node->next_edge(i).function.get();
+    while (n && runs(n)) {
+      if (auto* acc = dynamic_cast<torch::autograd::AccumulateGrad*>(n)) {
+        out.emplace_back((int64_t)i, acc);
+        break;
+      }
+      if (n->num_outputs() != 1 || !kept.count(n->name())) break;
+      n = n->next_edge(0).function.get();
+    }
+  }
+  return out;
+}
+static std::vector<Tensor> leaves_behind() {
+  std::vector<Tensor> out;
+  for (const auto& a : accumulators_behind()) out.push_back(a.second->variable);
+  return out;
+}
+// The first input that leads to an accumulator of another stream, or -1.
+static int64_t foreign_behind() {
+  for (const auto& a : accumulators_behind())
+    if (is_foreign(*a.second, a.second->variable)) return a.first;
   return -1;
 }
 
@@ -81,13 +129,14 @@ inline variable_list once(variable_list g, const char* who) {
   return (*err)(std::move(in));
 }
 
-inline void refuse_foreign(AutogradContext*, const std::vector<OptTensor>& leaves, const char* who) {
-  const int64_t i = foreign_leaf(leaves);
-  if (i >= 0)
+inline void refuse(int64_t input, const char* who) {
+  if (input >= 0)
     throw std::runtime_error(std::string(who) + ": a backward pass cannot be captured while an eager graph of the same leaves lives (input " +
-                             std::to_string(i) + " was used on another stream): drop that graph's outputs first, or run the warm-up on the "
+                             std::to_string(input) + " was used on another stream): drop that graph's outputs first, or run the warm-up on the "
                              "capture's stream");
 }
+inline void refuse_foreign(const std::vector<OptTensor>& leaves, const char* who) { refuse(foreign_leaf(leaves), who); }
+inline void refuse_foreign_behind(const char* who) { refuse(foreign_behind(), who); }
 
 struct Attn {
   Tensor q, k, v, table, cu_q, cu_k, map;
@@ -134,7 +183,7 @@ struct AttnNode : public torch::autograd::Function<AttnNode> {
     Attn a{s[0], s[1], s[2], s[3], s[4], s[5], s[6], ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool()};
     const Tensor &q = a.q, &k = a.k, &out = s[7], &stats = s[8], &rest = s[9];
     void* stream = (void*)ctx->saved_data["stream"].toInt();
-    if (g_text.capturing(stream)) refuse_foreign(ctx, {q, k, a.v, a.table.defined() ? OptTensor(a.table) : OptTensor()}, "attention_packed");
+    if (g_text.capturing(stream)) refuse_foreign_behind("attention_packed");
     const Tensor dout = rows(grad_out[0]);
     const int tq = (int)q.size(0), heads = (int)q.size(1), dim = (int)q.size(2), tk = (int)k.size(0), kv = (int)k.size(1);
     Tensor dq = at::empty({tq, heads, dim}, q.options()), dk = at::empty({tk, kv, dim}, q.options()), dv = at::empty({tk, kv, dim}, q.options());
@@ -162,7 +211,7 @@ Tensor attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, con
   const Tensor q = rows(q_in), k = rows(k_in), v = rows(v_in);           // (a copy of a leaf leads back to it: the leaves themselves are asked)
   const OptTensor table = table_in.has_value() ? OptTensor(table_in->contiguous()) : table_in;
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (table.has_value() && table->requires_grad()))) {
-    if (g_text.capturing((void*)stream)) refuse_foreign(nullptr, {q_in, k_in, v_in, table_in}, "attention_packed");
+    if (g_text.capturing((void*)stream)) refuse_foreign({q_in, k_in, v_in, table_in}, "attention_packed");
     return AttnNode::apply(q, k, v, table, cu_q, cu_k, map, causal, scale, stream);
   }
   return attn_forward(Attn{q, k, v, table.has_value() ? *table : Tensor(), cu_q, cu_k, map.has_value() ? *map : Tensor(), scale, causal}, nullptr, nullptr, (void*)stream);
@@ -197,7 +246,7 @@ struct RmsNode : public torch::autograd::Function<RmsNode> {
     const Tensor dh = grad_out.size() > 1 && grad_out[1].defined() ? grad_out[1].contiguous() : Tensor();
     if (!grad_out[0].defined() && !dh.defined()) return g;
     void* stream = (void*)ctx->saved_data["stream"].toInt();
-    if (g_text.capturing(stream)) refuse_foreign(ctx, {s[3], r.defined() ? OptTensor(r) : OptTensor(), w}, "rms_norm_residual");
+    if (g_text.capturing(stream)) refuse_foreign_behind("rms_norm_residual");
     const Tensor dy = grad_out[0].defined() ? grad_out[0].contiguous() : at::zeros_like(h);
     Tensor dx = at::empty_like(h), dw = at::empty_like(w);
     const int64_t cols = h.size(-1), rows = h.numel() / cols;
@@ -217,7 +266,7 @@ struct RmsNode : public torch::autograd::Function<RmsNode> {
 // x, residual (..., C) contiguous, weight (C,) contiguous, as rms_norm_residual has checked them -> [y, h] or [y]
 std::vector<Tensor> rms_norm(const Tensor& x, const OptTensor& r, const Tensor& w, double eps, int64_t stream) {
   if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (r.has_value() && r->requires_grad()))) {
-    if (g_text.capturing((void*)stream)) refuse_foreign(nullptr, {x, r, w}, "rms_norm_residual");
+    if (g_text.capturing((void*)stream)) refuse_foreign({x, r, w}, "rms_norm_residual");
     return RmsNode::apply(x, r, w, eps, stream);
   }
   Tensor y, h;
@@ -264,6 +313,8 @@ void bind_text(const std::unordered_map<std::string, int64_t>& p) {
 
 void register_text(pybind11::module& m) {
   m.def("foreign_leaf", &foreign_leaf);
+  m.def("foreign_behind", &foreign_behind);
+  m.def("leaves_behind", &leaves_behind);
   m.def("bind_text", &bind_text);
   m.def("attention", &attention);
   m.def("rms_norm", &rms_norm);

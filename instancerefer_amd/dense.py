@@ -501,7 +501,7 @@ class RMSNormFn(torch.autograd.Function):
             return None, None, None, None
         if torch.cuda.is_current_stream_capturing():
             from . import _nodes
-            _nodes.refuse_foreign_leaves("rms_norm_residual", _nodes.leaves_of(ctx))
+            _nodes.refuse_foreign_behind("rms_norm_residual")
         dy = torch.zeros_like(h) if dy is None else dy.contiguous()
         dh = None if dh is None else dh.contiguous()
         dx = torch.empty_like(h)
