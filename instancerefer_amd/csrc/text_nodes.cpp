@@ -232,7 +232,8 @@ struct RmsNode : public torch::autograd::Function<RmsNode> {
     const Tensor r = r_o.has_value() ? *r_o : Tensor();
     Tensor y, h, rstd;
     rms_forward(x, r, w, eps, &y, &h, &rstd, (void*)stream);
-    ctx->save_for_backward({h.defined() ? h : x, w, rstd, x, r});
+    ctx->save_for_backward({h.defined() ? h : x, w, rstd});              // (x and the residual are not read again)
+    ctx->saved_data["residual"] = r.defined();
     ctx->saved_data["stream"] = stream;
     ctx->set_materialize_grads(false);
     if (h.defined()) return {y, h};
@@ -242,7 +243,7 @@ struct RmsNode : public torch::autograd::Function<RmsNode> {
   static variable_list backward(AutogradContext* ctx, variable_list grad_out) {
     variable_list g(5);
     const auto s = ctx->get_saved_variables();
-    const Tensor &h = s[0], &w = s[1], &rstd = s[2], &r = s[4];
+    const Tensor &h = s[0], &w = s[1], &rstd = s[2];
     const Tensor dh = grad_out.size() > 1 && grad_out[1].defined() ? grad_out[1].contiguous() : Tensor();
     if (!grad_out[0].defined() && !dh.defined()) return g;
     void* stream = (void*)ctx->saved_data["stream"].toInt();
@@ -257,7 +258,7 @@ struct RmsNode : public torch::autograd::Function<RmsNode> {
           "irx_rms_norm_bwd");
     variable_list d = once({dx, dw}, "rms_norm_residual");
     g[0] = d[0];
-    if (r.defined()) g[1] = d[0];
+    if (ctx->saved_data["residual"].toBool()) g[1] = d[0];
     g[2] = d[1];
     return g;
   }
