@@ -42,7 +42,7 @@ struct AtTensor { const void* p; long long st, sh; };
 struct AtParams {
   AtTensor q, k, v, dout;                    // dout: backward only
   const void* out; const void* rest;         // backward: the output and, in 16 bits, what its rounding left (or NULL), laid out alike
-  const float* stats;                        // out [tq][heads][dim] contiguous; stats [heads][tq][2] = (row maximum * log2 e, 1 / row sum)
+  const float* stats;                        // out [tq][heads][dim] contiguous; stats [heads][tq][2] = (exponent of weight 1, 1 / sum of weights)
   void* dst; void* dst2;                     // fwd: out, its rounding's rest (may be NULL); dq kernel: dq; dk/dv kernel: dk, dv
   float* wstats;                             // fwd: stats (may be NULL)
   float* delta;                              // [heads][tq]: sum_d out * dout, written by the dq kernel, read by the dk/dv kernel
@@ -313,6 +313,12 @@ static inline int at_want_lds(const void* fn, size_t bytes, const char* who) {
 }
 
 #define IRX_LOG2E 1.44269504088896340736f
+
+// The forward's weights are 2^(s - m), m the exponent of weight 1: the running maximum less LIFT, moved only when a row's maximum outgrows it by
+// SLACK, so weights stay below 2^(LIFT + SLACK). float16 has 10 bits down to 2^-14, steps of 2^-24 below, and ends at 65504: with the row's
+// largest weight at 2^7 or more a weight is off by 2^-11 of itself or 2^-32 of the largest (unlifted 2^-25: where the heaviest key's value is
+// zero and 1000 keys at 2^-25 of it make the result, that was all of it). bf16 and float32 have the range.
+template <class T> struct AtLift { static constexpr float LIFT = T::ID == IRX_ATTN_F16 ? 7.f : 0.f, SLACK = T::ID == IRX_ATTN_F16 ? 4.f : 8.f; };
 
 // bias of one head by clipped distance, times log2 e, into LDS. A finite bias stays finite (the type's lowest value times log2 e would not).
 template <class T> __device__ __forceinline__ void at_load_bias(float* sb, const AtParams& P, int head) {

@@ -11,7 +11,8 @@
 // three waves per SIMD (207), the scores of the next tile beside the weights of this one (275; at dimension 64 without bias 10 % faster),
 // wave priorities around the matrix instructions (191), a zigzag order of the tiles (the same).
 // Exponents are base 2 (scale * log2 e is folded into one multiply-add per score); scores, weights' sums and the output are 32 bits, the
-// weights are rounded to the operand type for the second product (a relative 2^-9 / 2^-12 per weight, below the output's own rounding).
+// weights are rounded to the operand type for the second product, by at most a relative 2^-8 (bf16) or 2^-11 (float16; AtLift has the end of
+// its range) each, which is the output's own rounding's size.
 #include "irx_attn.h"
 
 // keys of a tile and workgroups per compute unit that the registers have to allow. 32 keys in float32: half the work where descriptions
@@ -147,8 +148,9 @@ __global__ __launch_bounds__(256, (fwd_waves<T, D>())) void k_attn_fwd(AtParams 
     for (int i = 1; i < N; ++i) mx = fmaxf(mx, s[i]);
     mx = at_pair_max(mx);
     if constexpr (!BIAS) mx *= c1;                                       // c1 > 0
-    // the running maximum moves only when a row outgrows it by 2^8: weights stay below 256, and most tiles rescale nothing
-    if (__any(mx > m + 8.f || m == -INFINITY)) {
+    mx -= AtLift<T>::LIFT;
+    // m moves only when a row outgrows it by SLACK: most tiles rescale nothing
+    if (__any(mx > m + AtLift<T>::SLACK || m == -INFINITY)) {
       const float mn = fmaxf(m, mx);
       const float a = mn == -INFINITY ? 1.f : at_exp2(m - mn);
       m = mn;
@@ -299,8 +301,8 @@ __global__ __launch_bounds__((64 * few_waves<T, D>())) void k_attn_few(AtParams 
     float mx = s[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-    mx = at_pair_max(mx) * c1;
-    if (__any(mx > m + 8.f || m == -INFINITY)) {
+    mx = at_pair_max(mx) * c1 - AtLift<T>::LIFT;
+    if (__any(mx > m + AtLift<T>::SLACK || m == -INFINITY)) {
       const float mn = fmaxf(m, mx);
       const float a = mn == -INFINITY ? 1.f : at_exp2(m - mn);
       m = mn;
