@@ -73,6 +73,94 @@ def _norm_table(dst, counts):
     return (ctypes.c_void_p * n)(*dst), c, n, int(_lib.load().irx_grad_gather_parts(c, n))
 
 
+# ---- which strided tensors share memory. Here a tensor is (first byte, element size, [(byte stride, length)] of its axes longer than one,
+# smallest stride first).
+def _axes(t):
+    e = t.element_size()
+    return t.data_ptr(), e, sorted((st * e, n) for st, n in zip(t.stride(), t.shape) if n > 1)
+
+
+def _reach(e, axes):
+    return e + sum((n - 1) * st for st, n in axes)
+
+
+def _runs(lo, e, axes, a, b):
+    """(starts in order, length) of the contiguous runs that reach into bytes [a, b)"""
+    run = e
+    while axes and axes[0][0] == run:
+        run, axes = run * axes[0][1], axes[1:]
+    at = np.array([lo], dtype=np.int64)
+    if axes:                                                    # of the widest axis only what can reach there
+        st, n = axes[-1]
+        at = lo + st * np.arange(n, dtype=np.int64)
+        at = at[(at + _reach(run, axes[:-1]) > a) & (at < b)]
+    for st, n in axes[:-1]:
+        at = (at[:, None] + st * np.arange(n, dtype=np.int64)).reshape(-1)
+    at = at[(at + run > a) & (at < b)]
+    at.sort()
+    return at, run
+
+
+def _itself(t):
+    """whether a tensor reaches a byte twice"""
+    lo, e, axes = t
+    if axes and axes[0][0] == 0:
+        return True
+    wide = e
+    for st, n in axes:
+        if st < wide:                                           # (axes inside each other never do)
+            at, run = _runs(lo, e, axes, lo, lo + _reach(e, axes))
+            return bool((np.diff(at) < run).any())
+        wide += st * (n - 1)
+    return False
+
+
+def _meet(x, y):
+    """whether two tensors share a byte: their contiguous runs where the ranges overlap"""
+    a, b = max(x[0], y[0]), min(x[0] + _reach(*x[1:]), y[0] + _reach(*y[1:]))
+    if a >= b:
+        return False
+    (p, n), (q, m) = _runs(*x, a, b), _runs(*y, a, b)
+    if not len(p) or not len(q):
+        return False
+    k = np.searchsorted(q, p)                                   # the run of q at or behind each run of p; the one before it
+    return bool((q[np.minimum(k, len(q) - 1)] - p < n)[k < len(q)].any() or (p - q[np.maximum(k - 1, 0)] < m)[k > 0].any())
+
+
+def _any_meet(group):
+    """whether two tensors of a group whose ranges overlap share memory. Pieces of one base (columns, every other row) lie at different
+    places between two steps of its widest stride; only what meets there is compared in full."""
+    wide, parts = max((st for _, _, axes in group for st, _ in axes), default=1), []
+    for t in group:
+        place = (t[0] % wide, t[1], [a for a in t[2] if a[0] % wide])
+        end = place[0] + _reach(*place[1:])
+        parts.append((place[0], end, place, t) if end <= wide else (0, wide, None, t))        # (None: it goes over the step's border)
+    parts.sort(key=lambda p: p[:2])
+    alive = []
+    for p in parts:
+        alive = [a for a in alive if a[1] > p[0]]
+        for a in alive:
+            if (a[2] is None or p[2] is None or _meet(a[2], p[2])) and _meet(a[3], p[3]):
+                return True
+        alive.append(p)
+    return False
+
+
+def _refuse_shared(grads):
+    """Raises if a tensor of the list reaches a value twice or two of them share memory."""
+    ts = sorted((_axes(g) for g in grads if g.numel()), key=lambda t: t[0])
+    if any(_itself(t) for t in ts):
+        raise ValueError("clip_grads_: a tensor that reaches a value more than once (expanded, windows) cannot be clipped in place")
+    groups, end = [], 0
+    for t in ts:
+        if t[0] >= end:
+            groups.append([])
+        groups[-1].append(t)
+        end = max(end, t[0] + _reach(*t[1:]))
+    if any(len(g) > 1 and _any_meet(g) for g in groups):
+        raise RuntimeError("clip_grads_: two tensors share memory")
+
+
 @torch.no_grad()
 def clip_grads_(grads, max_norm, norm_type=2.0):
     """Clip the GLOBAL norm of a list of gradients to max_norm, in place (csrc/irx_optim.hip): every value is multiplied by
@@ -80,13 +168,14 @@ def clip_grads_(grads, max_norm, norm_type=2.0):
     infinite where the gradients are, and a NaN norm makes every gradient NaN). For parameters held by FlatAdam use its
     backward_step(max_norm=...): no pass of its own over the gradients.
 
-    grads: dense float32, bfloat16 or float16 tensors on one device, mixed freely; None entries are skipped. No two may share memory.
+    grads: dense float32, bfloat16 or float16 tensors on one device, mixed freely, of any strides; None entries are skipped. No two may
+    share memory and none may reach a value twice (refused before anything is written).
     norm_type: 2 or inf."""
     max_norm, inf_norm = _clip_args("clip_grads_", max_norm, norm_type)
     grads = [grads] if isinstance(grads, torch.Tensor) else [g for g in grads if g is not None]
     if not grads:
         return torch.zeros(())
-    dev, back, flat = grads[0].device, [], []
+    dev, strided = grads[0].device, []
     for g in grads:
         if g.layout != torch.strided or g.dtype not in _CLIP_TYPES:
             raise ValueError("clip_grads_: dense float32, bfloat16 or float16 tensors, got %s of %s" % (g.layout, g.dtype))
@@ -94,13 +183,11 @@ def clip_grads_(grads, max_norm, norm_type=2.0):
             raise RuntimeError("irx operators need tensors on a HIP device (got %s); the CPU path exists only as the test oracle under /oracle" % g.device)
         if g.device != dev:
             raise ValueError("clip_grads_: tensors on %s and %s" % (dev, g.device))
-        if not (g.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(g)):      # any order of one gap-free range will do
-            if any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
-                raise ValueError("clip_grads_: an expanded tensor cannot be clipped in place")
-            c = g.contiguous()
-            back.append((g, c))
-            g = c
-        flat.append(g)
+        strided.append(not (g.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(g)))      # any order of one gap-free range will do
+    if any(strided):                                            # (gap-free ranges alone: the library compares them)
+        _refuse_shared(grads)
+    flat = [g.contiguous() if st else g for g, st in zip(grads, strided)]
+    back = [(g, c) for g, c, st in zip(grads, flat, strided) if st]
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return _clip(flat, back, max_norm, inf_norm)
