@@ -203,6 +203,7 @@ def _clip(flat, back, max_norm, inf_norm):
     ws = torch.empty(nb, dtype=torch.uint8, device=flat[0].device)
     norm = torch.empty((), dtype=torch.float32, device=flat[0].device)
     _lib.call("irx_clip_grads", ptrs, types, counts, n, inf_norm, max_norm, norm.data_ptr(), ws.data_ptr(), nb, _lib.stream_ptr())
+    torch.autograd.graph.increment_version(flat)                # written behind autograd's back
     for g, c in back:
         g.copy_(c)
     return norm
