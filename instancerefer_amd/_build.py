@@ -27,6 +27,8 @@ def _stale() -> bool:
     if not os.path.exists(LIB_PATH):
         return True
     t = os.path.getmtime(LIB_PATH)
+    if os.path.getmtime(os.path.abspath(__file__)) > t:        # the flags stand in this file
+        return True
     for f in SOURCES + HEADERS:
         if os.path.getmtime(os.path.join(CSRC, f)) > t:
             return True
@@ -91,7 +93,7 @@ def nodes_stale() -> bool:
     if not os.path.exists(NODES_PATH):
         return True
     t = os.path.getmtime(NODES_PATH)
-    return any(os.path.exists(f) and os.path.getmtime(f) > t for f in NODES_SRCS + NODES_HDRS)
+    return any(os.path.exists(f) and os.path.getmtime(f) > t for f in NODES_SRCS + NODES_HDRS + [os.path.abspath(__file__)])
 
 
 def build_nodes(force: bool = False, verbose: bool = False) -> str:
