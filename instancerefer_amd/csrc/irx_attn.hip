@@ -12,7 +12,7 @@
 // wave priorities around the matrix instructions (191), a zigzag order of the tiles (the same).
 // Exponents are base 2 (scale * log2 e is folded into one multiply-add per score); scores, weights' sums and the output are 32 bits, the
 // weights are rounded to the operand type for the second product, by at most a relative 2^-8 (bf16) or 2^-11 (float16; AtLift has the end of
-// its range) each, which is the output's own rounding's size.
+// its range) each, which is the output's own rounding's size; in short launches they go through it in two terms (fwd_two).
 #include "irx_attn.h"
 
 // keys of a tile and workgroups per compute unit that the registers have to allow. 32 keys in float32: half the work where descriptions
@@ -21,7 +21,8 @@
 template <class T, int D> constexpr int fwd_bn() { return T::ESZ == 4 ? 32 : 64; }
 template <class T, int D> constexpr int fwd_waves() { return T::ESZ == 4 && D == 128 ? 1 : 2; }
 
-template <class T, int D, bool BIAS>
+// TWO: a weight enters the second product in two terms, its rounding to 16 bits and the rounding of what that left over (fwd_two).
+template <class T, int D, bool BIAS, bool TWO>
 __global__ __launch_bounds__(256, (fwd_waves<T, D>())) void k_attn_fwd(AtParams P, int total) {
   constexpr int BN = fwd_bn<T, D>(), N = BN / 2;                        // keys of a tile, scores per lane
   typedef AtTile<T, D, BN> Tile;
@@ -171,8 +172,19 @@ __global__ __launch_bounds__(256, (fwd_waves<T, D>())) void k_attn_fwd(AtParams 
 #pragma unroll
     for (int ks = 0; ks < BN / 16; ++ks) {
       const F p = at_pack<T>(s + 8 * ks);
+      F rest = p;
+      if constexpr (TWO) {
+        float r[8];
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b) acc[b] = at_mma(Tile::col_frag(lv_, 16 * ks, b), p, acc[b]);
+        for (int e = 0; e < 8; ++e) r[e] = s[8 * ks + e] - at_get<T>(p, e);
+        rest = at_pack<T>(r);
+      }
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+        const F v = Tile::col_frag(lv_, 16 * ks, b);
+        acc[b] = at_mma(v, p, acc[b]);
+        if constexpr (TWO) acc[b] = at_mma(v, rest, acc[b]);
+      }
     }
   }
   l = at_pair_sum(l);
@@ -410,18 +422,34 @@ template <class T, int D> static int launch_few(AtParams P, int tokens, hipStrea
   return launch_join<T, D>(P, st);
 }
 
-template <class T, int D, bool BIAS> static int launch_fwd(const AtParams& P, hipStream_t st) {
+template <class T, int D, bool BIAS, bool TWO> static int launch_fwd(const AtParams& P, hipStream_t st) {
   const size_t lds = 4 * AtTile<T, D, fwd_bn<T, D>()>::BYTES + (BIAS ? sizeof(float) * (2 * P.far + 1) : 0);
   const long long total = (long long)P.slots * P.heads * P.splits;
   const unsigned grid = (unsigned)((total + 7) / 8 * 8);
-  if (int rc = at_want_lds(reinterpret_cast<const void*>(&k_attn_fwd<T, D, BIAS>), lds, "irx_attn_packed_fwd")) return rc;
-  k_attn_fwd<T, D, BIAS><<<grid, 256, lds, st>>>(P, (int)total);
+  if (int rc = at_want_lds(reinterpret_cast<const void*>(&k_attn_fwd<T, D, BIAS, TWO>), lds, "irx_attn_packed_fwd")) return rc;
+  k_attn_fwd<T, D, BIAS, TWO><<<grid, 256, lds, st>>>(P, (int)total);
   IRX_CHECK_LAUNCH("irx_attn_packed_fwd");
   return P.splits > 1 ? launch_join<T, D>(P, st) : IRX_OK;
 }
+
+// Two terms per weight where a 16-bit launch is short and leaves compute units without a workgroup: the output is then the exact one rounded once,
+// and the gradients' D = out . dout does not carry the weights' rounding into every dS, which shows most in short sequences (57 rows, dimension 128, bf16:
+// dq's error 1.51 times its own rounding, 1.41 with two terms). It costs nothing there but at the limit (256 rows, 64 heads, forward: dimension 64 9.4 us
+// both ways, dimension 128 10.4 and 11.4). Everywhere it would cost the matrix-bound launches 4 to 8 % of both passes (12289 causal rows, 8 heads of
+// 64, fp16: 900 and 972 us), and long rows average the weights' rounding out (dq 1.44 to 1.46, at dimension 32 1.49).
+static bool fwd_two(const AtParams& P) {
+  if (P.batch <= 0) return false;
+  const long long busy = P.batch < P.tq ? P.batch : P.tq;
+  return (P.tq / IRX_ATTN_BM + busy) * P.heads <= 256 && P.tk / P.batch <= 256;
+}
+template <class T, int D, bool BIAS> static int launch_fwd_t(const AtParams& P, hipStream_t st) {
+  if constexpr (T::ESZ == 2)
+    if (fwd_two(P)) return launch_fwd<T, D, BIAS, true>(P, st);
+  return launch_fwd<T, D, BIAS, false>(P, st);
+}
 template <class T, int D> static int launch_fwd_b(const AtParams& P, int tokens, hipStream_t st) {
   if (tokens) return launch_few<T, D>(P, tokens, st);
-  return P.table ? launch_fwd<T, D, true>(P, st) : launch_fwd<T, D, false>(P, st);
+  return P.table ? launch_fwd_t<T, D, true>(P, st) : launch_fwd_t<T, D, false>(P, st);
 }
 template <class T> static int launch_fwd_d(const AtParams& P, int dim, int tokens, hipStream_t st) {
   return dim == 32 ? launch_fwd_b<T, 32>(P, tokens, st) : dim == 64 ? launch_fwd_b<T, 64>(P, tokens, st) : launch_fwd_b<T, 128>(P, tokens, st);
