@@ -180,8 +180,11 @@ template <class T> __device__ __forceinline__ void at_st4(typename T::S* p, floa
   }
 }
 
-// the same, and what the rounding left over, rounded in its turn (rest == NULL: not wanted)
+// the same, and what the rounding left over, rounded in its turn (rest == NULL: not wanted). The values are products: float16 has an instruction
+// that multiplies and rounds at once, and where the compiler takes it for one of the two uses only, output and rest belong to different neighbours
+// of a value in the middle. So a value is a float register before either use.
 template <class T> __device__ __forceinline__ void at_st4_rest(typename T::S* p, typename T::S* rest, float a, float b, float c, float d) {
+  if constexpr (T::ID == IRX_ATTN_F16) asm("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
   at_st4<T>(p, a, b, c, d);
   if constexpr (T::ID == IRX_ATTN_BF16) {
     if (rest) {
