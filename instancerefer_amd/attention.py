@@ -15,13 +15,14 @@ over every key j of the sequence or, with `causal`, j <= i + Lk - Lq (the last q
 zeros and takes no gradient; so do rows outside every sequence (behind cu[-1]).
 
 Types: float32 (products in float32), bfloat16, float16; scores, softmax and sums are float32, the softmax's weights and the score gradients
-are rounded to the tensors' type where they enter the second products (in short launches the weights in two terms). In float16 a weight below 2^-21 of its row's largest keeps fewer than 10
-bits, one below 2^-32 none. In 16 bits a forward that will be differentiated keeps a second tensor
-of the output's size, what its rounding left over, for the gradients' sake. Float16 gradients of scores below 6e-8 vanish: scale the loss.
+are rounded to the tensors' type where they enter the second products (in short launches the weights in two terms). In float16 a weight below
+2^-21 of its row's largest keeps fewer than 10 bits, one below 2^-32 none; gradients of scores below 6e-8 vanish: scale the loss. In 16 bits a
+forward that will be differentiated keeps a second tensor of the output's size, what its rounding left over, for the gradients' sake. An
+exponent is good to 2^-22 of its score: weights of scores beyond 1e6 have no digits left, beyond 5e7 a row may come out as NaN or zeros.
 Keys of other sequences and rows outside never reach a result, whatever they hold. A NaN or infinity in a later row of the SAME sequence
 can reach earlier rows of its tile of 64 under `causal`, as in any matrix product. Head dimensions other than 32, 64 and 128 are padded to the
-next of them (a copy), up to 128. Deterministic; captures into a graph (the offsets may change between replays, the shapes may not). A capture with gradients is refused
-while an eager graph of the same leaves lives on another stream."""
+next of them (a copy), up to 128. Deterministic; captures into a graph (the offsets may change between replays, the shapes may not). A capture
+with gradients is refused while an eager graph of the same leaves lives on another stream."""
 import math
 import os
 

@@ -164,8 +164,8 @@ def _refuse_shared(grads):
 @torch.no_grad()
 def clip_grads_(grads, max_norm, norm_type=2.0):
     """Clip the GLOBAL norm of a list of gradients to max_norm, in place (csrc/irx_optim.hip): every value is multiplied by
-    min(1, max_norm / (norm + 1e-6)). Returns the norm before clipping as a 0-dim float32 tensor on their device (no host read; NaN or
-    infinite where the gradients are, and a NaN norm makes every gradient NaN). For parameters held by FlatAdam use its
+    min(1, max_norm / (norm + 1e-6)). Returns the norm before clipping as a 0-dim float32 tensor on their device (no host read; 0 on the
+    CPU for an empty list; NaN or infinite where the gradients are, and a NaN norm makes every gradient NaN). For parameters held by FlatAdam use its
     backward_step(max_norm=...): no pass of its own over the gradients.
 
     grads: dense float32, bfloat16 or float16 tensors on one device, mixed freely, of any strides; None entries are skipped. No two may
